@@ -65,6 +65,27 @@ class AhDecode(C.Structure):
                 ("wte", u64), ("wpe", u64), ("lnf_w", u64), ("lnf_b", u64), ("head", u64), ("kv", u64), ("logits", u64)]
 
 
+class AhPages(C.Structure):
+    _fields_ = [("dtype", i32), ("kv_heads", i32), ("head_dim", i32), ("page_rows", i32), ("seqs", i32), ("table_pages", i32), ("pages", i64),
+                ("page_stride", i64), ("row_stride", i64), ("head_stride", i64), ("k", u64), ("v", u64), ("table", u64), ("starts", u64), ("lens", u64)]
+
+
+class AhPagedAppend(C.Structure):
+    _fields_ = [("rows", i32), ("heads", i32), ("rot_dim", i32), ("rot_rows", i32), ("rot_neighbours", i32), ("reserved", i32),
+                ("q_st", i64), ("q_sh", i64), ("k_st", i64), ("k_sh", i64), ("v_st", i64), ("v_sh", i64), ("r_st", i64), ("r_sh", i64),
+                ("q", u64), ("k", u64), ("v", u64), ("rotated", u64), ("rotary", u64)]
+
+
+class AhPagedAttention(C.Structure):
+    _fields_ = [("rows", i32), ("heads", i32), ("scale", f32), ("soft_cap", f32), ("q_st", i64), ("q_sh", i64), ("o_st", i64), ("o_sh", i64),
+                ("q", u64), ("o", u64), ("lse", u64)]
+
+
+class AhSample(C.Structure):
+    _fields_ = [("dtype", i32), ("vocab", i32), ("rows", i64), ("ld", i64), ("logits", u64), ("temperature", u64), ("top_k", u64),
+                ("top_p", u64), ("min_p", u64), ("uniform", u64), ("tokens", u64), ("logprobs", u64)]
+
+
 class AhRng(C.Structure):
     _fields_ = [("s0", i32), ("s1", i32), ("has_spare", i32), ("_pad", i32), ("spare", C.c_double)]
 
@@ -157,6 +178,9 @@ SIGNATURES = {
     "ah_flash_fwd": [C.POINTER(AhFlash)], "ah_flash_bwd": [C.POINTER(AhFlash)],
     "ah_decode": [C.POINTER(AhDecode), C.POINTER(AhDecodeLayer), i32, i32], "ah_decode_head": [C.POINTER(AhDecode), u64],
     "ah_decode_stats": [p_i64, p_i64], "ah_decode_next_ticks": [i32],
+    "ah_paged_append": [C.POINTER(AhPages), C.POINTER(AhPagedAppend)],
+    "ah_paged_attention": [C.POINTER(AhPages), C.POINTER(AhPagedAttention)],
+    "ah_sample": [C.POINTER(AhSample)],
     "ah_adamw": [u64, u64, u64, u64, u64, C.POINTER(AhAdamW), u64, u64, u64],
     "ah_clip_coef": [u64, f32, f32, u64],
     "ah_side_begin": [], "ah_side_end": [], "ah_side_join": [],

@@ -489,6 +489,78 @@ int32_t ah_decode_stats(int64_t *one_launch, int64_t *again);
  * computed again; below: that computation is given up as well, and its logits are NaN. */
 int32_t ah_decode_next_ticks(int32_t ticks);
 
+/* ---- many sequences at once: their keys and values in pages, attention of their new tokens over those, and the next token of each.
+ *      sample() (packages/train/src/sample.ts:36-198) runs one sequence; with these a batch of them, of any lengths, goes through a
+ *      model together, some with a whole prompt or a chunk of one, some with one token.  No counterpart in the reference.
+ *
+ *      Position p of sequence s lies in row p % page_rows of page table[s][p / page_rows], feature d of head h of it at
+ *        k + page * page_stride + row * row_stride + h * head_stride + d       (elements; the same for v).
+ *      The new tokens of all sequences are one array of rows, those of sequence s the rows starts[s] .. starts[s + 1] - 1: its last
+ *      positions, of lens[s] in all.  Rows behind starts[seqs] belong to no sequence and stay as they are in every output.
+ *      table, starts and lens are read when the kernels run, so a captured graph follows what is written there.  What they hold is
+ *      checked there too, and nothing outside the arrays is touched: starts are taken into 0 .. rows; a position whose page is
+ *      outside 0 .. pages - 1 or past the table is not written, and attention that reads it gives NaN (output and lse).
+ *      A page may be shared by sequences; two new tokens must not fall on one row of a page.
+ *      All pointers 16-byte aligned (table, starts, lens, lse: 4), strides multiples of 16 bytes; head_dim a multiple of 8 from 8 to 128. ---- */
+typedef struct {
+  int32_t dtype;                 /* AH_F32 or AH_BF16: of the pages and of every q, k, v and o that meets them */
+  int32_t kv_heads, head_dim;
+  int32_t page_rows;             /* positions to a page: 1 .. 65536, any number */
+  int32_t seqs, table_pages;     /* sequences; entries that `table` has for each */
+  int64_t pages;                 /* pages in k and in v */
+  int64_t page_stride, row_stride, head_stride;
+  ah_ptr  k, v;
+  ah_ptr  table;                 /* i32 [seqs][table_pages] */
+  ah_ptr  starts, lens;          /* i32 [seqs + 1], i32 [seqs] */
+} AhPages;
+/* k and v of the new tokens go to their positions' places.  With a rotation (rot_dim > 0) features 0 .. rot_dim - 1 of q and k are
+ * turned by their position's angles on the way, and q, turned, goes to `rotated` (which may be q itself): pair i of a head, (i,
+ * i + rot_dim / 2) or with rot_neighbours (2 i, 2 i + 1), becomes (a cos - b sin, b cos + a sin) with the cosines in
+ * rotary[position][0 .. rot_dim / 2 - 1] and the sines behind them, in f32; rounded once.  A position past rot_rows - 1 gives NaN.
+ * Without one q, rotated and rotary are 0 and q is left alone. */
+typedef struct {
+  int32_t rows, heads;           /* rows of q, k, v; heads of q */
+  int32_t rot_dim;               /* even, at most head_dim; 0: no rotation */
+  int32_t rot_rows;              /* positions in `rotary` */
+  int32_t rot_neighbours, reserved;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, r_st, r_sh;    /* strides of a row and of a head in q, k, v and rotated (elements) */
+  ah_ptr  q, k, v, rotated, rotary;
+} AhPagedAppend;
+int32_t ah_paged_append(const AhPages *p, const AhPagedAppend *a);
+/* The new token at position i of its sequence attends to the sequence's positions 0 .. i, which ah_paged_append has stored:
+ *   s = scale q.k;  s = soft_cap tanh(s / soft_cap) if soft_cap > 0;  o = softmax(s) v;  lse = log(sum exp s).
+ * Head h of q goes with head h / (heads / kv_heads) of the pages.  What lies behind a token's position weighs nothing, infinite or NaN
+ * as it may be.  A token with no position to see (lens[s] below its sequence's number of new tokens) gets o = 0 and lse = -infinity. */
+typedef struct {
+  int32_t rows, heads;           /* rows of q and o; heads: a multiple of kv_heads */
+  float   scale, soft_cap;
+  int64_t q_st, q_sh, o_st, o_sh;
+  ah_ptr  q, o;
+  ah_ptr  lse;                   /* f32 [rows][heads]; 0: not wanted */
+} AhPagedAttention;
+int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *a);
+/* The next token of every row of logits from a given random number, as sample() chooses it on the host (sample.ts:85-193), with min-p:
+ *   temperature t <= 0 (or NaN): the first largest logit.  Otherwise, with w = exp((logit - largest) / t):
+ *   top_k k, if 0 < k < vocab, keeps the logits not below the k-th largest (equal ones stay);
+ *   top_p p, if 0 < p < 1, keeps of those, from the largest down (equal ones by index), as few as have p of their sum of w;
+ *   min_p m, if m > 0, keeps of those the ones with w >= m (of a largest w of 1).
+ * The token is the first whose running sum of w over what is kept passes uniform * that sum, from the largest down where top_p is
+ * on and by index where it is not (what the reference does); the last one if none does.  logprob = log(its w / that sum).
+ * NaN is never chosen; of infinite logits the largest are equal; a row without a logit above -infinity gives token 0 and logprob NaN.
+ * Sums are taken in 64-bit whole numbers: the same row gives the same token in every batch. */
+typedef struct {
+  int32_t dtype;                 /* of the logits: AH_F32 or AH_BF16 */
+  int32_t vocab;
+  int64_t rows, ld;              /* row stride in elements, at least vocab */
+  ah_ptr  logits;
+  ah_ptr  temperature;           /* f32 [rows]; 0: 1 */
+  ah_ptr  top_k, top_p, min_p;   /* i32, f32, f32 [rows]; 0: off */
+  ah_ptr  uniform;               /* f32 [rows] in [0, 1) */
+  ah_ptr  tokens;                /* out, i32 [rows] */
+  ah_ptr  logprobs;              /* out, f32 [rows]; 0: not wanted */
+} AhSample;
+int32_t ah_sample(const AhSample *s);
+
 /* ---- optimizer.  Backend.adamwStep (interfaces.ts:149-150; CPU loop optimizers.ts:76-92). ---- */
 typedef struct {
   float lr, beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale;

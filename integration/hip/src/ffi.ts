@@ -86,6 +86,8 @@ export const lib = dlopen(process.env.ALPHA_HIP_LIB ?? "libalpha_hip.so", {
   ah_layernorm_colsums:            { args: [ptr, i32], returns: i32 },
   ah_lion:                         { args: [u64, u64, u64, u64, ptr], returns: i32 },
   ah_masked_fill:                  { args: [u64, u64, u64, u64, u64, f32], returns: i32 },
+  ah_paged_append:                 { args: [ptr, ptr], returns: i32 },
+  ah_paged_attention:              { args: [ptr, ptr], returns: i32 },
   ah_pos_embedding_bwd:            { args: [u64, u64, i64, i64, i64, i32], returns: i32 },
   ah_probe_issue:                  { args: [i32, i32, i32, ptr], returns: i32 },
   ah_probe_mfma_bf16:              { args: [i32, i32, i32, ptr], returns: i32 },
@@ -96,6 +98,7 @@ export const lib = dlopen(process.env.ALPHA_HIP_LIB ?? "libalpha_hip.so", {
   ah_rng_next:                     { args: [ptr, ptr], returns: i32 },
   ah_rng_next_gauss:               { args: [ptr, ptr], returns: i32 },
   ah_rng_seed:                     { args: [ptr, i32], returns: i32 },
+  ah_sample:                       { args: [ptr], returns: i32 },
   ah_scale_inplace:                { args: [u64, f32, u64], returns: i32 },
   ah_scatter_slice:                { args: [u64, u64, i32, ptr, ptr, ptr], returns: i32 },
   ah_sgd:                          { args: [u64, u64, u64, f64, f64], returns: i32 },
@@ -149,6 +152,10 @@ export const LAYOUT = {
   AhCopy: { size: 32, dst: 0, src: 8, bytes: 16, value: 24 },
   AhDecode: { size: 96, vocab: 0, width: 4, heads: 8, ffn: 12, layers: 16, act: 20, rows: 24, scale: 28, cap: 32, eps: 36, wte: 40, wpe: 48, lnf_w: 56, lnf_b: 64, head: 72, kv: 80, logits: 88 },
   AhDecodeLayer: { size: 112, ln1_w: 0, ln1_b: 8, wqkv: 16, wo: 24, ln2_w: 32, ln2_b: 40, fc1: 48, up: 56, fc2: 64, coef: 72 },
+  AhPages: { size: 96, dtype: 0, kv_heads: 4, head_dim: 8, page_rows: 12, seqs: 16, table_pages: 20, pages: 24, page_stride: 32, row_stride: 40, head_stride: 48, k: 56, v: 64, table: 72, starts: 80, lens: 88 },
+  AhPagedAppend: { size: 128, rows: 0, heads: 4, rot_dim: 8, rot_rows: 12, rot_neighbours: 16, reserved: 20, q_st: 24, q_sh: 32, k_st: 40, k_sh: 48, v_st: 56, v_sh: 64, r_st: 72, r_sh: 80, q: 88, k: 96, v: 104, rotated: 112, rotary: 120 },
+  AhPagedAttention: { size: 72, rows: 0, heads: 4, scale: 8, soft_cap: 12, q_st: 16, q_sh: 24, o_st: 32, o_sh: 40, q: 48, o: 56, lse: 64 },
+  AhSample: { size: 88, dtype: 0, vocab: 4, rows: 8, ld: 16, logits: 24, temperature: 32, top_k: 40, top_p: 48, min_p: 56, uniform: 64, tokens: 72, logprobs: 80 },
   // GENERATED LAYOUTS END
 } as const;
 
