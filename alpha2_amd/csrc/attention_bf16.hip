@@ -20,7 +20,7 @@
 //     possible p, exp(-80), is far inside fp32 / bf16 range.  tanh' = 4r(1 - r) reuses r in the backward kernels;
 //   * masking code runs only for tiles that touch the diagonal or the end of the sequence (a wave-uniform branch);
 //   * constant factors (scale, the 4 of tanh') are applied once to the accumulators, not per score.
-#include "attention_common.h"
+#include "attention_bf16_tiles.h"
 #include <cstdlib>
 #include <cstring>
 
@@ -28,29 +28,11 @@ using namespace ah;
 
 namespace {
 
-constexpr int ST = 64;       // streamed rows per LDS tile
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) bf16x4 lds_v4;
-
-template <int D> struct Geo {
-  static constexpr int PITCH = D + 16;                 // bf16 elements; (D+16)*2 bytes = 32 mod 128 for D in {32,64,128}... see tile_frag_t
-  static constexpr int ELEMS = ST * PITCH;
-  static constexpr int CHUNKS = ST * D / 8 / 256;      // 16-byte chunks per thread per tile (D=32: 1, 64: 2, 128: 4)
-};
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float FIXED_MAX_CAP = 40.f;      // soft caps up to this use the constant-maximum softmax
 // AH_FLASH_BWD=onepass makes variant 1 of the backward pass the default of a process (measurement aid)
 bool flash_bwd_one_pass() {
   static const bool on = [] { const char *e = getenv("AH_FLASH_BWD"); return e && strcmp(e, "onepass") == 0; }();
   return on;
 }
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
-// First statement of a block that only the tiles on the diagonal need (masking): with it the compiler keeps the block behind a
-// branch the other tiles skip, where it would otherwise turn a cheap block into selects that every tile executes.
-__device__ __forceinline__ void keep_branch() { asm volatile("; rare path" ::: "memory"); }
 
 // global -> registers: rows [row0, row0+64) of a [T][D] operand with row stride st (elements); rows >= T read as zero
 // (PAD: the tensors' head size hd is smaller than D; features hd .. D - 1 read as zero)
@@ -64,36 +46,6 @@ __device__ __forceinline__ void tile_load(const uint16_t *__restrict__ base, int
     v[i] = x;
   }
 }
-template <int D>
-__device__ __forceinline__ void tile_store(uint16_t *s, const u32x4 (&v)[Geo<D>::CHUNKS]) {
-#pragma unroll
-  for (int i = 0; i < Geo<D>::CHUNKS; i++) {
-    int c = threadIdx.x + 256 * i, r = c / (D / 8), c8 = c % (D / 8);
-    *reinterpret_cast<u32x4 *>(s + r * Geo<D>::PITCH + c8 * 8) = v[i];
-  }
-}
-// A/B fragment with the tile ROW as the MFMA row/column (k = feature d): rows r0 + lane%32, d = 16*ks + 8*(lane/32)..
-template <int D>
-__device__ __forceinline__ bf16x8 tile_frag(const uint16_t *s, int r0, int ks, int lane) {
-  return *reinterpret_cast<const bf16x8 *>(s + (r0 + (lane & 31)) * Geo<D>::PITCH + ks * 16 + (lane >> 5) * 8);
-}
-// A fragment with the feature d as the MFMA row (k = tile row, in the accumulator's slot order): features
-// 32*db + lane%32, k-slot i of this half = tile row r0 + 16m + 8(i/4) + 4(lane/32) + i%4.
-template <int D>
-__device__ __forceinline__ bf16x8 tile_frag_t(const uint16_t *s, int r0, int m, int db, int lane) {
-  int j = lane & 15, g = lane >> 4, lk = g >> 1;
-  const uint16_t *p = s + (r0 + 16 * m + 4 * lk + (j >> 2)) * Geo<D>::PITCH + 32 * db + 16 * (g & 1) + 4 * (j & 3);
-  bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)p);
-  bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(p + 8 * Geo<D>::PITCH));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-// accumulator registers 8m..8m+7 -> bf16 B operand of MFMA m
-__device__ __forceinline__ bf16x8 acc_to_b(const f32x16 &s, int m) {
-  bf16x8 r;
-#pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = (__bf16)s[8 * m + i];
-  return r;
-}
 // this lane's row of a [T][D] operand as B fragments (k = d): one 16-byte global load per 16 features
 template <int D, bool PAD = false>
 __device__ __forceinline__ void row_frags(const uint16_t *__restrict__ base, int64_t st, int row, bool live, int lane, bf16x8 (&f)[D / 16], int hd = D) {
@@ -104,19 +56,6 @@ __device__ __forceinline__ void row_frags(const uint16_t *__restrict__ base, int
     f[ks] = __builtin_bit_cast(bf16x8, x);
   }
 }
-// O^T-style accumulators (rows = features 32db + 8j + 4h + r, column = owned row) -> bf16 row-major store
-template <int D, bool PAD = false>
-__device__ __forceinline__ void store_rows(uint16_t *__restrict__ dst, const f32x16 (&acc)[D / 32], float mul, int lane, int hd = D) {
-  int lk = lane >> 5;
-#pragma unroll
-  for (int db = 0; db < D / 32; db++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      uint2 w = make_uint2(pack_bf16x2(acc[db][4 * j] * mul, acc[db][4 * j + 1] * mul), pack_bf16x2(acc[db][4 * j + 2] * mul, acc[db][4 * j + 3] * mul));
-      if (!PAD || 32 * db + 8 * j + 4 * lk < hd) *reinterpret_cast<uint2 *>(dst + 32 * db + 8 * j + 4 * lk) = w;
-    }
-}
-
 // ------------------------------------------------------------------------------------------ forward
 // Launch bounds ask for at least two (three) waves per SIMD at head sizes up to 64: besides the occupancy this keeps the
 // register budget at 256 (170), where the compiler uses the VGPR form of MFMA and no accumulator ever has to be copied

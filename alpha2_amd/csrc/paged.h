@@ -25,13 +25,15 @@ inline Quotient quotient_by(uint32_t divisor) {
 }
 AH_BOTH uint32_t quotient(uint32_t n, const Quotient &q) { return (uint32_t)(((uint64_t)n * q.magic) >> q.shift); }
 
+constexpr int32_t MOST_POSITIONS = 0x7fff0000;      // so that a tile behind a position is still a position
+
 struct PagedCache {
   const int32_t *table, *starts, *lens;
   int64_t  pages, page_stride, row_stride, head_stride;
   Quotient page_rows;
   int32_t  seqs, table_pages;
   int32_t  rows;              // of the arrays of new tokens
-  int32_t  capacity;          // positions that the table can name, at most 2^31 - 1
+  int32_t  capacity;          // positions that the table can name, at most MOST_POSITIONS
 };
 
 // Elements from the start of a page array to (position, head 0), from the page that the table names for it; negative: no such place.

@@ -1,5 +1,5 @@
-// Keys and values in pages: appending those of new tokens, and attention over them (include/alpha_hip.h has the definitions).
-#include "attention_common.h"
+// Keys and values in pages: appending those of new tokens (ah_paged_append, include/alpha_hip.h).
+#include "common.h"
 #include "paged.h"
 
 using namespace ah;
@@ -24,7 +24,7 @@ int32_t paged_cache(const char *who, const AhPages *p, int32_t rows, PagedCache 
     AH_ARG(p->starts && p->lens && ((p->k && p->v && p->table) || p->pages == 0 || p->table_pages == 0), "%s: a null page array, table, starts or lens", who);
   const int64_t capacity = p->pages == 0 ? 0 : (int64_t)p->table_pages * p->page_rows;
   *out = PagedCache{dp<const int32_t>(p->table), dp<const int32_t>(p->starts), dp<const int32_t>(p->lens), p->pages, p->page_stride, p->row_stride, p->head_stride,
-                    quotient_by((uint32_t)p->page_rows), p->seqs, p->table_pages, rows, (int32_t)(capacity < INT32_MAX ? capacity : INT32_MAX)};
+                    quotient_by((uint32_t)p->page_rows), p->seqs, p->table_pages, rows, (int32_t)(capacity < MOST_POSITIONS ? capacity : MOST_POSITIONS)};
   return AH_OK;
 }
 
@@ -86,65 +86,6 @@ __global__ __launch_bounds__(64) void k_paged_append(AppendArgs a) {
   }
 }
 
-// ------------------------------------------------------------------------------------------ attention
-struct AttendArgs {
-  PagedCache c;
-  const void *k, *v, *q;
-  void *o;
-  float *lse;
-  int64_t q_st, q_sh, o_st, o_sh;
-  int32_t heads, group, head_dim;
-  float scale, cap;
-};
-
-// A workgroup of four waves to a row and head: each wave every fourth position, a feature (and the 64th behind it) to a lane.
-template <class T>
-__global__ __launch_bounds__(256) void k_paged_attention(AttendArgs a) {
-  const int row = blockIdx.x, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int position;
-  const int seq = sequence_at(a.c, row, position);
-  if (seq < 0) return;
-  const T *K = (const T *)a.k + (head / a.group) * a.c.head_stride, *V = (const T *)a.v + (head / a.group) * a.c.head_stride;
-  const T *Q = (const T *)a.q + row * a.q_st + head * a.q_sh;
-  const bool in0 = lane < a.head_dim, in1 = lane + 64 < a.head_dim;
-  const float q0 = in0 ? Io<T>::ld(Q, lane) : 0.f, q1 = in1 ? Io<T>::ld(Q, lane + 64) : 0.f;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int end = min(position + 1, a.c.capacity);
-  for (int p = wave; p < end; p += 4) {
-    const int64_t place = position_place(a.c, seq, p);
-    float s = NAN, v0 = 0.f, v1 = 0.f;
-    if (place >= 0) {
-      s = (in0 ? q0 * Io<T>::ld(K, place + lane) : 0.f) + (in1 ? q1 * Io<T>::ld(K, place + lane + 64) : 0.f);
-      if (in0) v0 = Io<T>::ld(V, place + lane);
-      if (in1) v1 = Io<T>::ld(V, place + lane + 64);
-    }
-    s = wave_sum(s) * a.scale;
-    if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
-    const float top = fmaxf(m, s), shift = top == -INFINITY ? 0.f : top;
-    const float keep = expf(m - shift), w = expf(s - shift);
-    l = l * keep + w;
-    o0 = o0 * keep + w * v0;
-    o1 = o1 * keep + w * v1;
-    m = top;
-  }
-  __shared__ float ms[4], ls[4], os[4][128];
-  if (lane == 0) { ms[wave] = m; ls[wave] = l; }
-  os[wave][lane] = o0;
-  os[wave][lane + 64] = o1;
-  __syncthreads();
-  const int f = threadIdx.x;
-  float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), sum = 0.f, o = 0.f;
-  const float shift = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < 4; w++) {
-    const float factor = expf(ms[w] - shift);
-    sum += ls[w] * factor;
-    if (f < 128) o += os[w][f] * factor;
-  }
-  if (position >= a.c.capacity) sum = NAN;          // positions that no table entry names
-  if (f < a.head_dim) Io<T>::st((T *)a.o + row * a.o_st + head * a.o_sh, f, sum == 0.f ? 0.f : o / sum);
-  if (f == 0 && a.lse) a.lse[(int64_t)row * a.heads + head] = sum == 0.f ? -INFINITY : top + logf(sum);
-}
-
 }  // namespace
 
 extern "C" {
@@ -176,27 +117,6 @@ int32_t ah_paged_append(const AhPages *p, const AhPagedAppend *d) {
   a.heads = d->rot_dim > 0 ? d->heads : 0; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
   a.rot = d->rot_dim; a.rot_rows = d->rot_rows; a.neighbours = d->rot_neighbours != 0;
   launch_kernel(p->dtype == AH_F32 ? k_paged_append<float> : k_paged_append<uint16_t>, dim3((unsigned)d->rows), dim3(64), 0, a);
-  AH_LAUNCH_CHECK();
-  return AH_OK;
-}
-
-int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *d) {
-  AH_ARG(d, "ah_paged_attention: no queries");
-  AttendArgs a{};
-  if (const int32_t rc = paged_cache("ah_paged_attention", p, d->rows, &a.c)) return rc;
-  const int64_t piece = p->dtype == AH_F32 ? 4 : 8;
-  AH_ARG(d->heads >= p->kv_heads && d->heads <= 65535 && d->heads % p->kv_heads == 0, "ah_paged_attention: %d heads are no multiple of the pages' %d", d->heads, p->kv_heads);
-  AH_ARG(d->q_st % piece == 0 && d->q_sh % piece == 0 && d->o_st % piece == 0 && d->o_sh % piece == 0 && aligned16(d->q) && aligned16(d->o) && d->lse % 4 == 0,
-         "ah_paged_attention: q and o of whole 16 bytes to a row and head");
-  AH_ARG(d->soft_cap >= 0.f && d->soft_cap < INFINITY && d->scale == d->scale, "ah_paged_attention: soft_cap %g, scale %g", d->soft_cap, d->scale);
-  AH_ARG(d->rows == 0 || p->seqs == 0 || (d->q && d->o), "ah_paged_attention: q or o is null");
-  AH_REQUIRE_READY();
-  if (d->rows == 0 || p->seqs == 0) return AH_OK;
-  a.k = dp<void>(p->k); a.v = dp<void>(p->v); a.q = dp<void>(d->q); a.o = dp<void>(d->o); a.lse = dp<float>(d->lse);
-  a.q_st = d->q_st; a.q_sh = d->q_sh; a.o_st = d->o_st; a.o_sh = d->o_sh;
-  a.heads = d->heads; a.group = d->heads / p->kv_heads; a.head_dim = p->head_dim;
-  a.scale = d->scale; a.cap = d->soft_cap;
-  launch_kernel(p->dtype == AH_F32 ? k_paged_attention<float> : k_paged_attention<uint16_t>, dim3((unsigned)d->rows, (unsigned)d->heads), dim3(256), 0, a);
   AH_LAUNCH_CHECK();
   return AH_OK;
 }

@@ -1,0 +1,904 @@
+// Attention of new tokens over keys and values in pages (ah_paged_attention, include/alpha_hip.h).
+//
+// Mathematics.  For a new token with limit n (the positions it sees, 0 .. n - 1):
+//   x_j = scale q.k_j (capped: cap tanh(x_j / cap)),  o = sum_j e^(x_j - m) v_j / sum_j e^(x_j - m),  lse = m + log sum_j e^(x_j - m)
+// in one pass over j with the running maximum m, sum l and product o, all in fp32; where the positions are cut into parts, each part leaves
+// its (m, l, o) and a second kernel joins them: m = max m_i, l = sum l_i e^(m_i - m), o = sum o_i e^(m_i - m).
+//
+// Work.  The heads that share keys are rows of one matrix: a COLUMN is a (new token, head of the group), column i of a sequence token
+// i / group, head i % group.  A workgroup takes one unit: TILE columns of a sequence, one kv head, one part of the positions.  Which unit that is
+// follows from starts and lens on the device (find_unit), so the lengths need not be known on the host, ragged batches are cut evenly
+// (parts are of one length for the whole launch, about the launch's work over the workgroups wanted) and a captured launch follows them.
+//
+// Two kernels for each type; both compute every case, which is taken is a matter of speed (ah_paged_attention):
+//   keys   16 columns; the four waves take tiles of positions in turn and are joined in LDS.  For one or a few new tokens a sequence, where the
+//          launch is bound by reading the pages once: 16 columns are the fewest that the matrix instructions take, most of them idle for one token.
+//   rows   the waves own columns and stream the same positions.  For chunks and prompts, bound by the matrix and vector pipes.
+//
+// Masked places.  A position past a column's limit has its score replaced by -infinity, whatever it was.  Its value would still meet a weight of 0
+// in the matrix product, and 0 x infinity is NaN; so rows past the part's end are zeros, and where some columns see a row that others do
+// not (tiles on the diagonal) values that are not finite are taken out of the product and put back by two products of 0s and 1s that count,
+// for each column, the +infinities (and NaN) and -infinities (and NaN) it does see.
+// A page that the table has wrong reads as NaN keys and zero values: whoever sees it gets NaN, nobody else.
+#include "attention_bf16_tiles.h"
+#include "paged.h"
+
+using namespace ah;
+
+namespace {
+
+struct Plan {
+  int32_t target;             // units that the positions of all tiles are cut into, about; 0: no cutting
+  int32_t least;              // positions of a part, at least
+  float  *parts;              // what the units of tiles with more than one part leave: see part_at
+};
+struct AttendArgs {
+  PagedCache c;
+  Plan plan;
+  const void *k, *v, *q;
+  void *o;
+  float *lse;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int32_t heads, kv_heads, group, head_dim;
+  float scale, cap;
+};
+
+struct Unit {
+  Sequence s;
+  int32_t seq, tile;          // -1: no such unit
+  int32_t part, parts;        // parts that hold positions which a column of the tile sees (at least one)
+  int32_t span;               // positions of a part
+  int32_t first;              // the tile's first unit
+  // the positions that column `i` of the sequence sees
+  __device__ __forceinline__ int limit(int i, int group) const { return s.len - s.count + i / group + 1; }
+};
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const Sequence &s, int group) { return (int)(((int64_t)s.count * group + TILE - 1) / TILE); }
+
+__device__ __forceinline__ int parts_of(int positions, int span) { return positions <= span ? 1 : (positions - 1) / span + 1; }
+
+// Unit `index` of the launch, or (by_tile) tile `index`, by a whole wave; the same for all its lanes.  A lane looks at a sequence.
+template <int TILE>
+__device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan, int group, int index, bool by_tile) {
+  const int lane = threadIdx.x & 63;
+  auto sequence = [&](int s) { return s < c.seqs ? sequence_of(c.starts[s], c.starts[s + 1], c.lens[s], c.rows) : Sequence{0, 0, 0}; };
+  Unit u;
+  u.seq = -1;
+  u.span = INT32_MAX;
+  Sequence mine = sequence(lane);
+  if (plan.target > 0) {
+    double work = 0;
+    for (int s0 = 0; s0 < c.seqs; s0 += 64) {
+      const Sequence s = s0 ? sequence(s0 + lane) : mine;
+      work += (double)tiles_of<TILE>(s, group) * min(s.len, c.capacity);
+    }
+    if (c.seqs > 1) work = wave_sum_d(work);
+    else work = __shfl(work, 0);
+    const double span = fmax(ceil(work / plan.target), (double)plan.least);
+    u.span = span < 2147483584.0 ? ((int)span + 63) / 64 * 64 : INT32_MAX;
+  }
+  int base = 0;
+  for (int s0 = 0; s0 < c.seqs; s0 += 64) {
+    if (s0) mine = sequence(s0 + lane);
+    const int reach = min(mine.len, c.capacity), tiles = tiles_of<TILE>(mine, group);
+    const int parts = parts_of(reach, u.span);
+    int count = by_tile ? tiles : tiles * parts, upto = count;
+    if (c.seqs > 1)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(upto, o); upto += lane >= o ? x : 0; }
+    const uint64_t past = __ballot(base + upto > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int before = base + __shfl(upto - count, at), p = __shfl(parts, at), n = __shfl(tiles, at);
+      u.s = Sequence{__shfl(mine.first, at), __shfl(mine.count, at), __shfl(mine.len, at)};
+      u.seq = s0 + at;
+      const int local = index - before, t = by_tile ? local : local / p;
+      u.tile = n - 1 - t;                                            // the last tiles of a prompt, which see most, come first
+      u.part = by_tile ? 0 : local - t * p;
+      u.first = by_tile ? 0 : before + t * p;
+      const int last = min((u.tile + 1) * TILE, u.s.count * group) - 1;
+      const int seen = min(u.limit(last, group), c.capacity);
+      u.parts = parts_of(seen, u.span);
+      // (by tile, the units before it are those of all tiles before it)
+      if (by_tile) u.first = t * p;
+      break;
+    }
+    base += __shfl(upto, 63);
+  }
+  return u;
+}
+
+// Where a unit's part is kept: TILE columns of D products, then TILE maxima, then TILE sums
+template <int TILE, int D>
+__device__ __forceinline__ float *part_at(const Plan &p, int64_t slot) { return p.parts + slot * (TILE * (D + 2)); }
+
+// ------------------------------------------------------------------------------------------ pages
+constexpr int64_t NO_PAGE = -1, NO_ROW = -2;         // a position whose page does not exist; one past the end
+// the table's entry for a position (0 where there is none to read)
+__device__ __forceinline__ int32_t page_entry(const PagedCache &c, const int32_t *__restrict__ table, int position, int end) {
+  return position < end ? table[quotient((uint32_t)position, c.page_rows)] : 0;
+}
+__device__ __forceinline__ int64_t place_of(const PagedCache &c, int32_t page, int position, int end) {
+  const uint32_t row = (uint32_t)position - quotient((uint32_t)position, c.page_rows) * c.page_rows.divisor;
+  const int64_t at = page_place(c, page, row);
+  return position < end ? at : NO_ROW;
+}
+constexpr uint32_t NAN_PAIR = 0x7fc07fc0u;
+__device__ __forceinline__ u32x4 piece_or(const uint16_t *base, int64_t place, int feature, bool inside, uint32_t missing) {
+  const uint32_t other = place == NO_PAGE && inside ? missing : 0u;
+  u32x4 x = {other, other, other, other};
+  if (place >= 0 && inside) x = *reinterpret_cast<const u32x4 *>(base + place + feature);
+  return x;
+}
+
+// ------------------------------------------------------------------------------------------ values that are not finite, bf16
+__device__ __forceinline__ bool has_special(bf16x8 v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) any |= (w[i] & 0x7f807f80u) + 0x00800080u;
+  return (any & 0x80008000u) != 0;
+}
+// v without them, and 1 where it is +infinity (-infinity) or NaN
+__device__ __forceinline__ void take_special(bf16x8 v, bf16x8 &rest, bf16x8 &up, bf16x8 &down) {
+  typedef __attribute__((ext_vector_type(8))) uint16_t u16x8;
+  const u16x8 w = __builtin_bit_cast(u16x8, v);
+  u16x8 r, p, n;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const bool special = (w[i] & 0x7f80) == 0x7f80;
+    r[i] = special ? 0 : w[i];
+    p[i] = special && w[i] != 0xff80 ? 0x3f80 : 0;
+    n[i] = special && w[i] != 0x7f80 ? 0x3f80 : 0;
+  }
+  rest = __builtin_bit_cast(bf16x8, r); up = __builtin_bit_cast(bf16x8, p); down = __builtin_bit_cast(bf16x8, n);
+}
+__device__ __forceinline__ bf16x8 ones_where_seen(bf16x8 p) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = (float)p[i] == 0.f ? (__bf16)0.f : (__bf16)1.f;
+  return r;
+}
+__device__ __forceinline__ float put_back(float o, float up, float down) { return o + (up > 0.f ? INFINITY : 0.f) + (down > 0.f ? -INFINITY : 0.f); }
+
+// ------------------------------------------------------------------------------------------ joining
+// The finished column: o and lse, or one unit's part of them.  m in units of `natural` (its logarithm's base), l the sum of weights.
+__device__ __forceinline__ float column_sum(float l, int limit, int reach) { return limit > reach ? NAN : l; }      // a position that no table entry names
+template <class T> __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<float>(float *p, float a, float b, float c, float d) { *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d); }
+template <> __device__ __forceinline__ void store4<uint16_t>(uint16_t *p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
+constexpr float LN2 = 0.693147180559945309f;
+
+// Joins the parts of a tile: a workgroup to a tile and kv head, a thread to four features of a column.  Maxima are logarithms to base 2.
+template <class T, int TILE, int D>
+__global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
+  const int head = blockIdx.x % a.kv_heads;
+  // the units of the tiles before this one have to be known: find_unit by tile gives those of the sequence, the others are added up here
+  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, true);
+  if (u.seq < 0 || u.parts == 1) return;
+  int before = 0;
+  for (int s0 = 0; s0 < u.seq; s0 += 64) {
+    const int s = s0 + (threadIdx.x & 63);
+    if (s < u.seq) {
+      const Sequence x = sequence_of(a.c.starts[s], a.c.starts[s + 1], a.c.lens[s], a.c.rows);
+      before += tiles_of<TILE>(x, a.group) * parts_of(min(x.len, a.c.capacity), u.span);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
+  const int64_t first = before + u.first;
+  const int columns = u.s.count * a.group;
+  for (int e = threadIdx.x; e < TILE * D / 4; e += 256) {
+    const int col = e / (D / 4), f = e % (D / 4) * 4, i = u.tile * TILE + col;
+    if (i >= columns || f >= a.head_dim) continue;
+    float m = -INFINITY;
+    for (int p = 0; p < u.parts; p++) m = fmaxf(m, part_at<TILE, D>(a.plan, (first + p) * a.kv_heads + head)[TILE * D + col]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < u.parts; p++) {
+      const float *part = part_at<TILE, D>(a.plan, (first + p) * a.kv_heads + head);
+      const float w = exp2_fast(part[TILE * D + col] - shift);
+      const float4 x = *reinterpret_cast<const float4 *>(part + col * D + f);
+      l = fmaf(part[TILE * D + TILE + col], w, l);
+      o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    }
+    l = column_sum(l, u.limit(i, a.group), a.c.capacity);
+    const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    store4<T>((T *)a.o + row * a.o_st + h * a.o_sh + f, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (f == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
+  }
+}
+
+// ------------------------------------------------------------------------------------------ keys, bf16
+// v_mfma_f32_16x16x32_bf16: S^T[32 positions, 16 columns] = K Q^T in two halves of 16, a lane holding positions 16 i + 4 g + r (g = lane / 16, r < 4) of column
+// lane % 16.  Those are, as they lie, the B operand of O^T[16 features, 16 columns] += V^T P^T when its slot 8 g + 4 i + r is taken to mean that
+// position; the A operand is read from V's tile in the same order (ds_read_b64_tr_b16 of four rows).  K goes from the pages straight into its operand's
+// registers (16 rows of 64 bytes to an instruction), V through LDS that is the wave's own, so that no wave waits for another before the end.
+template <int D> struct KeysTile {
+  static constexpr int PITCH = D + 16, V_BYTES = 32 * PITCH * 2, O_PITCH = D + 4, O_BYTES = 16 * O_PITCH * 4;
+  static constexpr int WAVE_BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
+};
+
+template <int D, bool CAPPED>
+__global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
+  using G = KeysTile<D>;
+  constexpr int KS = D / 32, DB = D / 16, NV = D / 16, TILE = 16;
+  __shared__ __attribute__((aligned(16))) char own[4 * G::WAVE_BYTES];
+  __shared__ float tops[4][TILE], sums[4][TILE];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % a.kv_heads;
+  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
+  if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
+  const int columns = u.s.count * a.group, i = u.tile * TILE + col, last = min((u.tile + 1) * TILE, columns) - 1;
+  const int limit = i < columns ? u.limit(i, a.group) : 0;
+  const int least = u.limit(u.tile * TILE, a.group);                 // every column sees the positions before this one
+  const int begin = u.parts > 1 ? u.part * u.span : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
+  const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
+  const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
+  uint16_t *tile = (uint16_t *)(own + wave * G::WAVE_BYTES);
+
+  bf16x8 q[KS];
+  {
+    const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
+    const uint16_t *p = (const uint16_t *)a.q + row * a.q_st + h * a.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      u32x4 x = {0u, 0u, 0u, 0u};
+      if (i < columns && ks * 32 + g * 8 < a.head_dim) x = *reinterpret_cast<const u32x4 *>(p + ks * 32 + g * 8);
+      q[ks] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+  // CAPPED: e^(2 x / cap) = 2^(c1 s), and the score in base 2 is c2 - 2 c2 / (that + 1); otherwise it is c1 s
+  const float c1 = CAPPED ? 2.0f * a.scale * LOG2E / a.cap : a.scale * LOG2E, c2 = a.cap * LOG2E;
+  f32x4 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  u32x4 kr[2][KS], vr[NV];
+  auto load = [&](int32_t page, int base) {        // a tile's rows: lane r (and r + 32) looks after position base + r
+    const int64_t place = place_of(a.c, page, base + (lane & 31), end);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int64_t at = __shfl(place, 16 * h + col);
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) kr[h][ks] = piece_or(K, at, ks * 32 + g * 8, ks * 32 + g * 8 < a.head_dim, NAN_PAIR);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int c = lane + 64 * n, f = c % (D / 8) * 8;
+      vr[n] = piece_or(V, __shfl(place, c / (D / 8)), f, f < a.head_dim, 0u);
+    }
+  };
+  const int stride = 4 * 32;
+  int base = begin + wave * 32;
+  int32_t page = page_entry(a.c, table, base + (lane & 31), end), next = page_entry(a.c, table, base + stride + (lane & 31), end);
+  if (base < end) load(page, base);
+  for (; base < end; base += stride) {
+    bf16x8 k[2][KS];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) k[h][ks] = __builtin_bit_cast(bf16x8, kr[h][ks]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");           // the tile's last reads are done
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int c = lane + 64 * n;
+      *reinterpret_cast<u32x4 *>(tile + c / (D / 8) * G::PITCH + c % (D / 8) * 8) = vr[n];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (base + stride < end) {
+      page = next;
+      next = page_entry(a.c, table, base + 2 * stride + (lane & 31), end);
+      load(page, base + stride);
+    }
+    f32x4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[h][ks], q[ks], s[h], 0, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[h][r] = CAPPED ? fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[h][r] * c1) + 1.0f), c2) : s[h][r] * c1;
+    const bool edge = base + 32 > min(least, end);
+    if (edge) {
+      keep_branch();
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[h][r] = base + 16 * h + 4 * g + r < min(limit, end) ? s[h][r] : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    top = max_lane<16>(max_lane<32>(top));
+    if (__any(top > m)) {
+      const float larger = fmaxf(m, top), keep = exp2_fast(m - (larger == -INFINITY ? 0.f : larger));
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[d][r] *= keep;
+      m = larger;
+    }
+    const float shift = m == -INFINITY ? 0.f : m;
+    bf16x8 p;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float w = exp2_fast(s[h][r] - shift);
+        l += w;
+        p[4 * h + r] = (__bf16)w;
+      }
+    auto values = [&](int d) {
+      const uint16_t *at = tile + (4 * g + (col >> 2)) * G::PITCH + 16 * d + 4 * (col & 3);
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(at + 16 * G::PITCH));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    bool special = false;
+    if (edge && least < end) {                                       // some columns see less than others
+      keep_branch();
+#pragma unroll
+      for (int d = 0; d < DB; d++) special |= has_special(values(d));
+      special = __any(special);
+    }
+    if (!special) {
+#pragma unroll
+      for (int d = 0; d < DB; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), p, o[d], 0, 0, 0);
+    } else {
+      const bf16x8 seen_p = ones_where_seen(p);
+      for (int d = 0; d < DB; d++) {
+        bf16x8 rest, up, down;
+        take_special(values(d), rest, up, down);
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const f32x4 ups = __builtin_amdgcn_mfma_f32_16x16x32_bf16(up, seen_p, zero, 0, 0, 0), downs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(down, seen_p, zero, 0, 0, 0);
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < DB; e++) x = e == d ? o[e] : x;
+        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rest, p, x, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = put_back(x[r], ups[r], downs[r]);
+#pragma unroll
+        for (int e = 0; e < DB; e++) o[e] = e == d ? x : o[e];
+      }
+    }
+  }
+
+  // the four waves: weights relative to the largest of their maxima
+  l = add_lane<16>(add_lane<32>(l));
+  if (g == 0) { tops[wave][col] = m; sums[wave][col] = l; }
+  __syncthreads();
+  {
+    const float top = fmaxf(fmaxf(tops[0][col], tops[1][col]), fmaxf(tops[2][col], tops[3][col]));
+    const float w = exp2_fast(m - (top == -INFINITY ? 0.f : top));
+    float *mine = (float *)(own + wave * G::WAVE_BYTES) + col * G::O_PITCH + 4 * g;
+#pragma unroll
+    for (int d = 0; d < DB; d++) *reinterpret_cast<float4 *>(mine + 16 * d) = make_float4(o[d][0] * w, o[d][1] * w, o[d][2] * w, o[d][3] * w);
+  }
+  __syncthreads();
+  float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
+  for (int e = threadIdx.x; e < TILE * D / 4; e += 256) {
+    const int c = e / (D / 4), f = e % (D / 4) * 4, ci = u.tile * TILE + c;
+    if (ci >= columns || f >= a.head_dim) continue;
+    const float top = fmaxf(fmaxf(tops[0][c], tops[1][c]), fmaxf(tops[2][c], tops[3][c])), shift = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float4 y = *reinterpret_cast<const float4 *>((const float *)(own + w * G::WAVE_BYTES) + c * G::O_PITCH + f);
+      sum = fmaf(sums[w][c], exp2_fast(tops[w][c] - shift), sum);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    if (u.parts > 1) {
+      *reinterpret_cast<float4 *>(part + c * D + f) = x;
+      if (f == 0) { part[TILE * D + c] = top; part[TILE * D + TILE + c] = sum; }
+    } else {
+      sum = column_sum(sum, u.limit(ci, a.group), a.c.capacity);
+      const int64_t row = u.s.first + ci / a.group, h = (int64_t)head * a.group + ci % a.group;
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      store4<uint16_t>((uint16_t *)a.o + row * a.o_st + h * a.o_sh + f, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      if (f == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.f ? -INFINITY : fmaf(top, LN2, logf(sum));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ rows, bf16
+// Four waves of 32 columns on v_mfma_f32_32x32x16_bf16, K and V in LDS in tiles of 64 positions, two of them in turn (one barrier to a tile), the next tile's
+// rows on their way in registers and the table's entries for the one behind that.  MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself
+// for the maximum (attention_bf16.hip); 2: a larger cap.
+template <int D>
+struct RowsPlaces {                                  // where this thread's pieces of a tile lie
+  static constexpr int N = Geo<D>::CHUNKS;
+  static __device__ __forceinline__ int row(int n) { return (threadIdx.x + 256 * n) / (D / 8); }
+  static __device__ __forceinline__ int feature() { return threadIdx.x % (D / 8) * 8; }
+};
+
+template <int D, int MODE>
+__device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
+  constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = RowsPlaces<D>::N;
+  constexpr bool CAPPED = MODE == 1;
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][Geo<D>::ELEMS], Vs[2][Geo<D>::ELEMS];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
+  const int head = blockIdx.x % a.kv_heads;
+  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
+  if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
+  const int columns = u.s.count * a.group, i0 = u.tile * TILE + wave * 32, i = i0 + lr;
+  const int limit = i < columns ? u.limit(i, a.group) : 0;
+  const int last = min((u.tile + 1) * TILE, columns) - 1, wave_last = min(i0 + 31, columns - 1);
+  const int begin = u.parts > 1 ? u.part * u.span : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
+  const int wave_end = wave_last < i0 ? 0 : min(u.limit(wave_last, a.group), end), least = u.limit(min(i0, columns - 1), a.group);
+  const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
+  const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
+  const float c1 = (MODE ? 2.0f * a.scale * LOG2E / a.cap : a.scale * LOG2E), c2 = a.cap * LOG2E;
+  const float ic2 = MODE ? -1.0f / (2.0f * c2) : 0.f;                // p = 2^(-2 c2 r) and -2 c2 r = 1 / ((e + 1) ic2)
+
+  bf16x8 qf[KS];
+  const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) {
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (i < columns && ks * 16 + lk * 8 < a.head_dim) x = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + row * a.q_st + h * a.q_sh + ks * 16 + lk * 8);
+    qf[ks] = __builtin_bit_cast(bf16x8, x);
+  }
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+  float m = CAPPED ? c2 : -INFINITY, l = 0.f;
+
+  u32x4 rk[N], rv[N];
+  int32_t entry[N];
+  const int feature = RowsPlaces<D>::feature();
+  const bool inside = feature < a.head_dim;
+  auto entries = [&](int base) {
+#pragma unroll
+    for (int n = 0; n < N; n++) entry[n] = page_entry(a.c, table, base + RowsPlaces<D>::row(n), end);
+  };
+  auto load = [&](int base) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const int64_t at = place_of(a.c, entry[n], base + RowsPlaces<D>::row(n), end);
+      rk[n] = piece_or(K, at, feature, inside, NAN_PAIR);
+      rv[n] = piece_or(V, at, feature, inside, 0u);
+    }
+  };
+  entries(begin);
+  load(begin);
+  entries(begin + ST);
+  tile_store<D>(Ks[0], rk);
+  tile_store<D>(Vs[0], rv);
+  __syncthreads();
+  int cur = 0;
+  for (int base = begin; base < end; base += ST, cur ^= 1) {
+    if (base + ST < end) {
+      load(base + ST);
+      entries(base + 2 * ST);
+    }
+#pragma unroll
+    for (int sub = 0; sub < ST / 32; sub++) {
+      const int kv0 = base + sub * 32;
+      if (kv0 >= wave_end) continue;                                 // (the same for the wave) nothing for its columns
+      f32x16 s;
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag<D>(Ks[cur], sub * 32, ks, lane), qf[ks], s, 0, 0, 0);
+      const bool edge = kv0 + 32 > min(least, end);
+      if (MODE == 1) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = exp2_fast(rcp_fast(fmaf(exp2_fast(s[e] * c1), ic2, ic2)));
+        if (edge) {
+          keep_branch();
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < min(limit, end) ? s[e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) l += s[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = MODE == 2 ? fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[e] * c1) + 1.0f), c2) : s[e] * c1;
+        if (edge) {
+          keep_branch();
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < min(limit, end) ? s[e] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+        top = max_lane<32>(top);
+        if (__any(top > m)) {
+          const float larger = fmaxf(m, top), keep = exp2_fast(m - (larger == -INFINITY ? 0.f : larger));
+          l *= keep;
+#pragma unroll
+          for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] *= keep;
+          m = larger;
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int e = 0; e < 16; e++) { s[e] = exp2_fast(s[e] - shift); l += s[e]; }
+      }
+      const bf16x8 p0 = acc_to_b(s, 0), p1 = acc_to_b(s, 1);
+      bool special = false;
+      if (edge && least < end) {                                     // some columns see less than others
+        keep_branch();
+#pragma unroll
+        for (int d = 0; d < DB; d++) special |= has_special(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane)) | has_special(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane));
+        special = __any(special);
+      }
+      if (!special) {
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane), p0, o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane), p1, o[d], 0, 0, 0);
+        }
+      } else {
+        const bf16x8 seen0 = ones_where_seen(p0), seen1 = ones_where_seen(p1);
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          f32x16 ups, downs;
+#pragma unroll
+          for (int e = 0; e < 16; e++) { ups[e] = 0.f; downs[e] = 0.f; }
+          bf16x8 rest, up, down;
+          take_special(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane), rest, up, down);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, p0, o[d], 0, 0, 0);
+          ups = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen0, ups, 0, 0, 0);
+          downs = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen0, downs, 0, 0, 0);
+          take_special(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane), rest, up, down);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, p1, o[d], 0, 0, 0);
+          ups = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen1, ups, 0, 0, 0);
+          downs = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen1, downs, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[d][e] = put_back(o[d][e], ups[e], downs[e]);
+        }
+      }
+    }
+    if (base + ST < end) {
+      tile_store<D>(Ks[cur ^ 1], rk);
+      tile_store<D>(Vs[cur ^ 1], rv);
+    }
+    __syncthreads();
+  }
+  l = add_lane<32>(l);
+  if (CAPPED && l == 0.f) m = -INFINITY;
+  if (i >= columns) return;
+  if (u.parts > 1) {
+    float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
+    const int c = wave * 32 + lr;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        *reinterpret_cast<float4 *>(part + c * D + 32 * d + 8 * j + 4 * lk) = make_float4(o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]);
+    if (lk == 0) { part[TILE * D + c] = m; part[TILE * D + TILE + c] = l; }
+    return;
+  }
+  l = column_sum(l, limit, a.c.capacity);
+  store_rows<D, true>((uint16_t *)a.o + row * a.o_st + h * a.o_sh, o, l == 0.f ? 0.f : 1.0f / l, lane, a.head_dim);
+  if (lk == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
+}
+template <int D, int MODE>
+__global__ __launch_bounds__(256, D <= 32 ? 3 : D <= 64 ? 2 : 1) void k_paged_rows_bf16(AttendArgs a) { paged_rows_bf16_body<D, MODE>(a); }
+
+// ------------------------------------------------------------------------------------------ fp32
+// v_mfma_f32_16x16x4_f32, nothing through LDS before the end: a tile is 16 positions, S^T[16 positions, 16 columns] = K Q^T, whose slot g of
+// instruction (j, c) is taken to mean feature 16 j + 4 g + c, so that both operands are 16-byte loads; a lane then holds positions 4 g + r of column
+// lane % 16, the B operand of O^T += V^T P^T whose slot g of instruction r means that position, and the A operand's row n of block (h, c) is taken
+// to mean feature W (16 h + n) + c with W = min(4, D / 16), so that V's pieces are 16-byte loads (8 at D = 32) of whole rows too.
+// SPLIT: 16 columns, the waves take tiles in turn and are joined (keys).  Otherwise every wave has NC times 16 columns of its own and streams all
+// positions; what one wave reads the others find in the caches (rows).
+// a score through the cap: cap tanh(x), x = score / cap
+__device__ __forceinline__ float capped_f32(float x, float cap) { return cap * (fabsf(x) < TANH_SMALL ? tanh_small(x) : tanh_large(x)); }
+
+template <int D, int NC, bool SPLIT>
+__device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
+  constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = SPLIT ? 16 : 64 * NC, O_PITCH = D + 4;
+  static_assert(!SPLIT || NC == 1, "one block of columns where the waves share them");
+  __shared__ __attribute__((aligned(16))) float joined[SPLIT ? 4 * 16 * O_PITCH : 4];
+  __shared__ float tops[4][16], sums[4][16];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int head = blockIdx.x % a.kv_heads;
+  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
+  if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
+  const int columns = u.s.count * a.group, i0 = u.tile * TILE + (SPLIT ? 0 : wave * 16 * NC);
+  const int last = min((u.tile + 1) * TILE, columns) - 1;
+  const int begin = u.parts > 1 ? u.part * u.span : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
+  const int wave_last = SPLIT ? last : min(i0 + 16 * NC - 1, columns - 1);
+  const int wave_end = wave_last < i0 ? 0 : min(u.limit(wave_last, a.group), end), least = u.limit(min(i0, columns - 1), a.group);
+  const float *K = (const float *)a.k + head * a.c.head_stride, *V = (const float *)a.v + head * a.c.head_stride;
+  const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
+  const float factor = a.cap > 0.f ? a.scale / a.cap : a.scale;
+
+  int limit[NC];
+  f32x4 q[NC][KQ], o[NC][DB];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int n = 0; n < NC; n++) {
+    const int i = i0 + 16 * n + col;
+    limit[n] = i < columns ? min(u.limit(i, a.group), end) : 0;
+    const float *p = (const float *)a.q + (u.s.first + (int64_t)(i / a.group)) * a.q_st + ((int64_t)head * a.group + i % a.group) * a.q_sh;
+#pragma unroll
+    for (int j = 0; j < KQ; j++) {
+      q[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (i < columns && 16 * j + 4 * g < a.head_dim) q[n][j] = *reinterpret_cast<const f32x4 *>(p + 16 * j + 4 * g);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; d++) o[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+  }
+
+  f32x4 kr[KQ];
+  float vr[4][VH][W];
+  auto load = [&](int32_t page, int base) {           // lane l looks after position base + l % 16
+    const int64_t place = place_of(a.c, page, base + col, end);
+#pragma unroll
+    for (int j = 0; j < KQ; j++) {
+      const bool inside = 16 * j + 4 * g < a.head_dim;
+      const float other = place == NO_PAGE && inside ? NAN : 0.f;
+      kr[j] = f32x4{other, other, other, other};
+      if (place >= 0 && inside) kr[j] = *reinterpret_cast<const f32x4 *>(K + place + 16 * j + 4 * g);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int64_t at = __shfl(place, 4 * g + r);
+#pragma unroll
+      for (int h = 0; h < VH; h++) {
+        const int f = W * (16 * h + col);
+        typedef __attribute__((ext_vector_type(W))) float piece;
+        piece x;
+#pragma unroll
+        for (int c = 0; c < W; c++) x[c] = 0.f;
+        if (at >= 0 && f < a.head_dim) x = *reinterpret_cast<const piece *>(V + at + f);
+#pragma unroll
+        for (int c = 0; c < W; c++) vr[r][h][c] = x[c];
+      }
+    }
+  };
+  const int stride = SPLIT ? 64 : 16;
+  int base = begin + (SPLIT ? wave * 16 : 0);
+  int32_t next = page_entry(a.c, table, base + stride + col, end);
+  if (base < wave_end) load(page_entry(a.c, table, base + col, end), base);
+  for (; base < wave_end; base += stride) {
+    f32x4 k[KQ];
+    float v[4][VH][W];
+#pragma unroll
+    for (int j = 0; j < KQ; j++) k[j] = kr[j];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int h = 0; h < VH; h++)
+#pragma unroll
+        for (int c = 0; c < W; c++) v[r][h][c] = vr[r][h][c];
+    if (base + stride < wave_end) {
+      const int32_t page = next;
+      next = page_entry(a.c, table, base + 2 * stride + col, end);
+      load(page, base + stride);
+    }
+    const bool edge = base + 16 > min(least, end);
+    bool special = false;
+    if (edge && least < end) {                        // some columns see less than others
+      keep_branch();
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int h = 0; h < VH; h++)
+#pragma unroll
+          for (int c = 0; c < W; c++) special |= !(fabsf(v[r][h][c]) < INFINITY);
+      special = __any(special);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+      f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KQ; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][c], q[n][j][c], s, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[r] *= factor;
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[r] = capped_f32(s[r], a.cap);
+      }
+      if (edge) {
+        keep_branch();
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[r] = base + 4 * g + r < limit[n] ? s[r] : -INFINITY;
+      }
+      float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      top = max_lane<16>(max_lane<32>(top));
+      if (__any(top > m[n])) {
+        const float larger = fmaxf(m[n], top), keep = exp2_fast((m[n] - (larger == -INFINITY ? 0.f : larger)) * LOG2E);
+        l[n] *= keep;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[n][d][r] *= keep;
+        m[n] = larger;
+      }
+      const float shift = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+      for (int r = 0; r < 4; r++) { s[r] = exp2_fast((s[r] - shift) * LOG2E); l[n] += s[r]; }
+      if (!special) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int h = 0; h < VH; h++)
+#pragma unroll
+            for (int c = 0; c < W; c++) o[n][W * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][h][c], s[r], o[n][W * h + c], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int h = 0; h < VH; h++)
+#pragma unroll
+          for (int c = 0; c < W; c++) {
+            f32x4 ups = {0.f, 0.f, 0.f, 0.f}, downs = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const float x = v[r][h][c], one = s[r] == 0.f ? 0.f : 1.f;
+              const bool fine = fabsf(x) < INFINITY;
+              o[n][W * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(fine ? x : 0.f, s[r], o[n][W * h + c], 0, 0, 0);
+              ups = __builtin_amdgcn_mfma_f32_16x16x4f32(!fine && !(x < 0.f) ? 1.f : 0.f, one, ups, 0, 0, 0);
+              downs = __builtin_amdgcn_mfma_f32_16x16x4f32(!fine && !(x > 0.f) ? 1.f : 0.f, one, downs, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[n][W * h + c][r] = put_back(o[n][W * h + c][r], ups[r], downs[r]);
+          }
+      }
+    }
+  }
+  // a lane has features W (16 h + 4 g + r) + c of its column in element r of block W h + c
+  if constexpr (!SPLIT) {
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+      const float sum = add_lane<16>(add_lane<32>(l[n]));
+      const int i = i0 + 16 * n + col;
+      if (i >= columns) continue;
+      float *to, mul = 1.f;
+      bool inside = true;
+      if (u.parts > 1) {
+        float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
+        const int c = wave * 16 * NC + 16 * n + col;
+        to = part + c * D;
+        if (g == 0) { part[TILE * D + c] = m[n] * LOG2E; part[TILE * D + TILE + c] = sum; }
+      } else {
+        const float all = column_sum(sum, u.limit(i, a.group), a.c.capacity);
+        const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
+        to = (float *)a.o + row * a.o_st + h * a.o_sh;
+        mul = all == 0.f ? 0.f : 1.0f / all;
+        inside = false;
+        if (g == 0 && a.lse) a.lse[row * a.heads + h] = all == 0.f ? -INFINITY : m[n] + logf(all);
+      }
+#pragma unroll
+      for (int h = 0; h < VH; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int f = W * (16 * h + 4 * g + r);
+          if (!inside && f >= a.head_dim) continue;
+#pragma unroll
+          for (int c = 0; c < W; c += 2) *reinterpret_cast<float2 *>(to + f + c) = make_float2(o[n][W * h + c][r] * mul, o[n][W * h + c + 1][r] * mul);
+        }
+    }
+  } else {
+    const float mine = add_lane<16>(add_lane<32>(l[0]));
+    if (g == 0) { tops[wave][col] = m[0]; sums[wave][col] = mine; }
+    __syncthreads();
+    {
+      const float top = fmaxf(fmaxf(tops[0][col], tops[1][col]), fmaxf(tops[2][col], tops[3][col]));
+      const float w = exp2_fast((m[0] - (top == -INFINITY ? 0.f : top)) * LOG2E);
+      float *to = joined + (wave * 16 + col) * O_PITCH;
+#pragma unroll
+      for (int h = 0; h < VH; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int c = 0; c < W; c++) to[W * (16 * h + 4 * g + r) + c] = o[0][W * h + c][r] * w;
+    }
+    __syncthreads();
+    float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
+    for (int e = threadIdx.x; e < 16 * D / 4; e += 256) {
+      const int c = e / (D / 4), f = e % (D / 4) * 4, ci = u.tile * TILE + c;
+      if (ci >= columns || f >= a.head_dim) continue;
+      const float top = fmaxf(fmaxf(tops[0][c], tops[1][c]), fmaxf(tops[2][c], tops[3][c])), shift = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const float4 y = *reinterpret_cast<const float4 *>(joined + (w * 16 + c) * O_PITCH + f);
+        sum = fmaf(sums[w][c], exp2_fast((tops[w][c] - shift) * LOG2E), sum);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      if (u.parts > 1) {
+        *reinterpret_cast<float4 *>(part + c * D + f) = x;
+        if (f == 0) { part[TILE * D + c] = top * LOG2E; part[TILE * D + TILE + c] = sum; }
+      } else {
+        sum = column_sum(sum, u.limit(ci, a.group), a.c.capacity);
+        const int64_t row = u.s.first + ci / a.group, h = (int64_t)head * a.group + ci % a.group;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        store4<float>((float *)a.o + row * a.o_st + h * a.o_sh + f, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        if (f == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.f ? -INFINITY : top + logf(sum);
+      }
+    }
+  }
+}
+template <int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_keys_f32(AttendArgs a) { paged_f32_body<D, 1, true>(a); }
+template <int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_rows_f32(AttendArgs a) { paged_f32_body<D, 2, false>(a); }
+
+// ------------------------------------------------------------------------------------------ launches
+// Parts go through the library's scratch (64 MB from ah_init on, ordered with everything else on the main stream), of which a launch takes at most this.
+constexpr int64_t PART_BYTES = int64_t(60) << 20;
+
+// TILE columns to a unit: how many workgroups, and how many of them the positions are cut for.  `wanted` workgroups fill the GPU; where the tiles alone
+// are as many there is nothing to cut, and the join is not launched either where the table cannot name more positions than a part has.
+template <class T, int TILE, int D, class Kernel>
+int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
+  const int64_t tiles = cdiv((int64_t)a.c.rows * a.group, TILE) + a.c.seqs;                  // of one kv head, at most
+  const int64_t slot = (int64_t)TILE * (D + 2) * sizeof(float) * a.kv_heads;
+  int64_t target = 0;
+  if (tiles * a.kv_heads < wanted && a.c.capacity > least) {
+    target = cdiv(wanted, a.kv_heads);
+    if ((tiles + target) * slot > PART_BYTES) target = PART_BYTES / slot - tiles;
+    if (target < 1) target = 0;
+  }
+  if (target > 0) {
+    a.plan.target = (int32_t)target;
+    a.plan.least = least;
+    a.plan.parts = (float *)scratch((size_t)((tiles + target) * slot));
+    if (!a.plan.parts) return fail(AH_ERR_OOM, "ah_paged_attention: no scratch for the parts of long sequences");
+  }
+  const int64_t grid = (tiles + target) * a.kv_heads;
+  if (grid > INT32_MAX) return fail(AH_ERR_UNSUPPORTED, "ah_paged_attention: %lld workgroups", (long long)grid);
+  launch_kernel(kernel, dim3((unsigned)grid), dim3(256), 0, a);
+  AH_LAUNCH_CHECK();
+  if (target > 0) {
+    launch_kernel(k_paged_join<T, TILE, D>, dim3((unsigned)(tiles * a.kv_heads)), dim3(256), 0, a);
+    AH_LAUNCH_CHECK();
+  }
+  return AH_OK;
+}
+template <int D>
+int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
+  const bool rows = (int64_t)a.c.rows * a.group > (int64_t)32 * a.c.seqs;                    // columns of a sequence, in the mean
+  const int64_t cus = num_cus();
+  if (bf16_pages) {
+    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 4 * cus, 256);
+    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 512);
+  }
+  if (!rows) return attend<float, 16, D>(a, k_paged_keys_f32<D>, 4 * cus, 256);
+  return attend<float, 128, D>(a, k_paged_rows_f32<D>, 2 * cus, 512);
+}
+
+}  // namespace
+
+extern "C" int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *d) {
+  AH_ARG(d, "ah_paged_attention: no queries");
+  AttendArgs a{};
+  if (const int32_t rc = paged_cache("ah_paged_attention", p, d->rows, &a.c)) return rc;
+  const int64_t piece = p->dtype == AH_F32 ? 4 : 8;
+  AH_ARG(d->heads >= p->kv_heads && d->heads <= 65535 && d->heads % p->kv_heads == 0, "ah_paged_attention: %d heads are no multiple of the pages' %d", d->heads, p->kv_heads);
+  AH_ARG((int64_t)d->rows * (d->heads / p->kv_heads) <= INT32_MAX / 2, "ah_paged_attention: %d rows of %d heads to a kv head", d->rows, d->heads / p->kv_heads);
+  AH_ARG(d->q_st % piece == 0 && d->q_sh % piece == 0 && d->o_st % piece == 0 && d->o_sh % piece == 0 && aligned16(d->q) && aligned16(d->o) && d->lse % 4 == 0,
+         "ah_paged_attention: q and o of whole 16 bytes to a row and head");
+  AH_ARG(d->soft_cap >= 0.f && d->soft_cap < INFINITY && d->scale == d->scale, "ah_paged_attention: soft_cap %g, scale %g", d->soft_cap, d->scale);
+  AH_ARG(d->rows == 0 || p->seqs == 0 || (d->q && d->o), "ah_paged_attention: q or o is null");
+  AH_REQUIRE_READY();
+  if (d->rows == 0 || p->seqs == 0) return AH_OK;
+  a.k = dp<void>(p->k); a.v = dp<void>(p->v); a.q = dp<void>(d->q); a.o = dp<void>(d->o); a.lse = dp<float>(d->lse);
+  a.q_st = d->q_st; a.q_sh = d->q_sh; a.o_st = d->o_st; a.o_sh = d->o_sh;
+  a.heads = d->heads; a.kv_heads = p->kv_heads; a.group = d->heads / p->kv_heads; a.head_dim = p->head_dim;
+  a.scale = d->scale; a.cap = d->soft_cap;
+  const bool bf16_pages = p->dtype == AH_BF16;
+  return p->head_dim <= 32 ? attend_sized<32>(a, bf16_pages) : p->head_dim <= 64 ? attend_sized<64>(a, bf16_pages) : attend_sized<128>(a, bf16_pages);
+}
