@@ -1,7 +1,7 @@
 """The next token from logits and given random numbers (ah_sample) against the definition in 64 bits.
 
-Tokens have to be equal.  The kernel's weights are whole numbers of 2^-43 of the largest, so a running sum of n of them is off by n 2^-44 at most
-(and as much by the exponential's last place): where the given number falls nearer than 2 n 2^-43 to a border between two tokens, or the
+Tokens have to be equal.  The kernel's weights are whole numbers of 2^-43 of the largest, from an exponential good to 2^-43, so a running sum of n of them is off by n (2^-44 + 2^-43)
+at most: where the given number falls nearer than 2 n 2^-43 to a border between two tokens, or the
 nucleus ends that near to one, either may be chosen; the cases below are looked at for that (`margin`) and are never so near.
 logprob: its exponent and the logarithm of the sum are taken in 64 bits and rounded once, 2^-24 of its value, and the sum is off by the above."""
 import ctypes as C
@@ -197,6 +197,22 @@ def test_peaked_and_flat_rows(B, dev, dtype):
     for k, p in ((0, 1.0), (0, 0.9013), (100, 1.0), (3000, 0.7003)):
         u = (rs.randint(0, 4000, 8) / 4000 + 0.0001237).astype(np.float32)
         check(B, dev, dtype, logits, np.full(8, 0.9), np.full(8, k), np.full(8, p), None, u)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_logits_that_lie_closer_or_wider_than_bins_can_tell(B, dev, dtype):
+    """Neighbouring numbers, the smallest ones and the largest ones, thousands of each; a step of a row's temperature is none of theirs."""
+    rs = np.random.RandomState(9)
+    V = 9001
+    pick = lambda *v: np.asarray(v, np.float32)[rs.randint(0, len(v), V)]
+    x = np.stack([pick(0.0, 1e-45, -1e-45), pick(3.4e38, -3.4e38, 0.0), pick(1.0, 1.0 + 2.0 ** -23, 1.0 - 2.0 ** -24), pick(-np.inf, 5.0, 5.0 + 2.0 ** -21),
+                  np.where(rs.random_sample(V) < 0.001, 1e5, rs.standard_normal(V) * 1e-3).astype(np.float32), pick(7.0, -1e30, 7.0 - 1e-3)])
+    logits = to_bf16(x) if dtype == ffi.BF16 else x
+    if dtype == ffi.BF16:
+        logits[3] = np.where(np.isneginf(x[3]), 0xff80, logits[3])
+    for t, k, p in ((1.0, 0, 0.6007), (1e-3, 0, 0.9003), (1.0, 3000, 1.0), (1e-3, 4500, 0.7013), (1.0, 30, 0.5003)):
+        u = (rs.randint(0, 4000, 6) / 4000 + 0.0001237).astype(np.float32)
+        check(B, dev, dtype, logits, np.full(6, t, np.float32), np.full(6, k), np.full(6, p), None, u)
 
 
 def test_the_choice_is_that_of_the_sampling_loop(B, dev):
