@@ -25,7 +25,6 @@ struct SampleArgs {
   int32_t vocab;
 };
 
-// (512 threads: with 1024 the 128 registers that each then has do not hold a row's state)
 constexpr int THREADS = 512, WAVES = THREADS / 64, BINS = 2048, LIST = 2048, EACH = LIST / THREADS, STEPS = 256;
 static_assert(BINS == LIST, "EACH bins, or entries, to a thread");
 constexpr int MAX_VOCAB = 1 << 20;              // sums of as many weights of 2^43 stay below 2^63
@@ -147,7 +146,6 @@ struct Past {                                    // a running sum, on from `base
   uint64_t base = 0;
   __device__ __forceinline__ bool operator()(uint64_t s) const { const double x = (double)(base + s); return reach ? x >= target : x > target; }
 };
-struct Found { float logit; int index; uint64_t upto; };     // upto: the running sum with it
 
 template <class T> struct Row {
   static constexpr int N = 16 / sizeof(T);       // logits to a vector
@@ -159,42 +157,73 @@ template <class T> struct Row {
     V = vocab;
     vectors = (lead + V + N - 1) / N;
   }
-  // vector v, NaN for what is not the row's (which is not read)
-  __device__ __forceinline__ void load(int v, float (&l)[N]) const {
-    if (v > 0 && v < vectors - 1) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(x + (int64_t)v * N);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < N; i++) l[i] = N == 4 ? __uint_as_float(u[i]) : __uint_as_float(i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
-    } else {
+  __device__ __forceinline__ int index(int v, int i) const { return v * N + i - lead; }
+  __device__ __forceinline__ float at(int index) const { return Io<T>::ld(x, (size_t)(index + lead)); }
+  // vector v as it is stored; what is not the row's is not read, and NaN
+  __device__ __forceinline__ uint4 load(int v) const {
+    uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
+    if (v > 0 && v < vectors - 1) w = *reinterpret_cast<const uint4 *>(x + (int64_t)v * N);
+    else if (v < vectors) {
+      uint32_t u[4] = {~0u, ~0u, ~0u, ~0u};
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        const int index = v * N + i - lead;
-        l[i] = NAN;
-        if (index >= 0 && index < V) l[i] = Io<T>::ld(x, (size_t)(index + lead));
+        const bool in = index(v, i) >= 0 && index(v, i) < V;
+        if (in) {
+          if constexpr (N == 4) u[i] = __float_as_uint(at(index(v, i)));
+          else {
+            const uint32_t half = __float_as_uint(at(index(v, i))) >> 16;
+            u[i / 2] = i & 1 ? (u[i / 2] & 0xffffu) | half << 16 : (u[i / 2] & 0xffff0000u) | half;
+          }
+        }
       }
+      w = make_uint4(u[0], u[1], u[2], u[3]);
     }
+    return w;
   }
-  // f(logit, index) for every logit above -infinity, U vectors under way at a time
+  static __device__ __forceinline__ float logit(const uint4 &w, int i) {
+    const uint32_t u = (N == 4 ? i : i / 2) == 0 ? w.x : (N == 4 ? i : i / 2) == 1 ? w.y : (N == 4 ? i : i / 2) == 2 ? w.z : w.w;
+    return N == 4 ? __uint_as_float(u) : __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+  }
+  // f(vector, its number) for all of them, U loads under way at a time
   template <int U, class F>
   __device__ __forceinline__ void each(F f) const {
     for (int v0 = threadIdx.x; v0 < vectors; v0 += THREADS * U) {
-      float l[U][N];
+      uint4 w[U];
 #pragma unroll
-      for (int j = 0; j < U; j++) if (v0 + j * THREADS < vectors) load(v0 + j * THREADS, l[j]);
+      for (int j = 0; j < U; j++) w[j] = load(v0 + j * THREADS);
 #pragma unroll
-      for (int j = 0; j < U; j++) if (v0 + j * THREADS < vectors)
+      for (int j = 0; j < U; j++) if (v0 + j * THREADS < vectors) f(w[j], v0 + j * THREADS);
+    }
+  }
+  // f(logit, index) for the ones above -infinity for which `hit` holds, which are few: the loop over them is there once
+  template <class Hit, class F>
+  __device__ __forceinline__ void hits(Hit hit, F f) const {
+    constexpr int U = 4;
+    for (int v0 = threadIdx.x; v0 < vectors; v0 += THREADS * U) {
+      uint4 w[U];
 #pragma unroll
-        for (int i = 0; i < N; i++) if (l[j][i] > -INFINITY) f(l[j][i], (v0 + j * THREADS) * N + i - lead);
+      for (int j = 0; j < U; j++) w[j] = load(v0 + j * THREADS);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < U; j++)
+#pragma unroll
+        for (int i = 0; i < N; i++) { const float l = logit(w[j], i); bits |= l > -INFINITY && hit(l) ? 1u << (j * N + i) : 0u; }
+      while (bits) {
+        const int b = __builtin_ctz(bits);
+        const int n = index(v0 + b / N * THREADS, b % N);
+        f(at(n), n);
+        bits &= bits - 1;
+      }
     }
   }
 };
 
-// weights against `top` at a temperature
+// weights against `top` at a temperature, as whole numbers; or 1 each
 struct Weight {
   float top;
   double factor;                                 // 256 log2(e) / temperature
   const double *steps;
+  bool one;
   __device__ __forceinline__ uint64_t operator()(float l) const {
     const double y = ((double)l - (double)top) * factor;
     const bool some = y > -44.0 * STEPS;         // (NaN: both are infinite)
@@ -207,62 +236,10 @@ struct Weight {
     const double step = steps[n & (STEPS - 1)], w = fma(step, e, step);
     const uint64_t scaled = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(int64_t)((n >> 8) + 43) << 52);
     const uint64_t units = __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52) - __builtin_bit_cast(uint64_t, 0x1p52);
-    return some ? units : l == top ? (uint64_t)UNIT : 0;
+    const uint64_t weight = some ? units : l == top ? (uint64_t)UNIT : 0;
+    return one ? 1 : weight;
   }
 };
-
-// The first by index at which the running sum of term(logit, index) passes; there is one.
-template <class T, class Term>
-__device__ __forceinline__ Found across(const Row<T> &row, Shared &s, Term term, Past past) {
-  constexpr int N = Row<T>::N;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, runs = (row.vectors + 63) / 64;
-  __syncthreads();
-  for (int r = wave; r < runs; r += WAVES) {
-    uint64_t sum = 0;
-    const int v = r * 64 + lane;
-    if (v < row.vectors) {
-      float l[N];
-      row.load(v, l);
-#pragma unroll
-      for (int i = 0; i < N; i++) if (l[i] > -INFINITY) sum += term(l[i], v * N + i - row.lead);
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) s.runs[r] = sum;
-  }
-  __syncthreads();
-  const int each = (runs + THREADS - 1) / THREADS, r0 = threadIdx.x * each;
-  uint64_t sum = 0, all;
-  for (int i = 0; i < each; i++) sum += r0 + i < runs ? s.runs[r0 + i] : 0;
-  uint64_t before = block_before(sum, s, all);
-  for (int i = 0; i < each; i++) {
-    const uint64_t x = r0 + i < runs ? s.runs[r0 + i] : 0;
-    if (!past(before) && past(before + x)) { s.found = r0 + i; s.found_before = before; }
-    before += x;
-  }
-  __syncthreads();
-  Found f{0.f, 0, 0};
-  const int v = same(s.found) * 64 + lane;       // every wave does the same
-  const uint64_t start = same(s.found_before);
-  float l[N];
-  uint64_t w[N];
-  sum = 0;
-#pragma unroll
-  for (int i = 0; i < N; i++) { l[i] = NAN; w[i] = 0; }
-  if (v < row.vectors) row.load(v, l);
-#pragma unroll
-  for (int i = 0; i < N; i++) { if (l[i] > -INFINITY) w[i] = term(l[i], v * N + i - row.lead); sum += w[i]; }
-  uint64_t upto = start + wave_running(sum) - sum;
-  bool here = false;
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    if (!past(upto) && past(upto + w[i])) { here = true; f = Found{l[i], v * N + i - row.lead, past.base + upto + w[i]}; }
-    upto += w[i];
-  }
-  const uint64_t who = __ballot(here);
-  const int from = who ? __builtin_ctzll(who) : 0;
-  return Found{same(__shfl(f.logit, from)), same(__shfl(f.index, from)), same((uint64_t)__shfl(f.upto, from))};
-}
 
 // Which of the bins between `high` and `low` a logit falls into: never an earlier one for a smaller logit.  A row's own bins are of one width, over `most`
 // at most; those of a bin are of one number of floats, so that they end as single ones whatever the logits are.
@@ -307,78 +284,17 @@ __device__ __forceinline__ void find_bin(Shared &s, int level, uint64_t base, co
   __syncthreads();
 }
 
-// Running sums of term(logit) over the bins, of the logits between `low` and `high`, into s.bins[level]; the sum of all
-template <class T, class Term>
-__device__ __forceinline__ uint64_t fill_bins(const Row<T> &row, Shared &s, int level, const Bins &bin, float low, float high, Term term) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += THREADS) s.bins[level][i] = 0;
-  __syncthreads();
-  row.template each<2>([&](float l, int) {
-    if (l >= low && l <= high) {
-      const uint64_t w = term(l);
-      if (w) atomicAdd((unsigned long long *)&s.bins[level][bin(l)], (unsigned long long)w);
-    }
-  });
-  __syncthreads();
-  return sum_bins(s, level);
-}
-
-// The first, from the largest down, at which the running sum of term(logit) passes; there is one.  s.bins[0] has the running sums of the logits between
-// `low` and `high` in `bin`.
-template <class T, class Term>
-__device__ __forceinline__ Found descend(const Row<T> &row, Shared &s, Bins bin, float low, float high, Term term, Past past) {
-  uint64_t base = 0;
-  __syncthreads();
-  // (the row's own bins, and at most three times those of a bin: 2^32 floats are 2^11 times 2^21, 2^10, 1.  Bounded as it stands, whatever the sums
-  // are: every wave takes the same turns, since all of them read what decides from the same places between the same two barriers.)
-  for (int cut = 0; cut < 5; cut++) {
-    const int level = cut ? 1 : 0;
-    if (threadIdx.x == 0) s.listed = 0;
-    find_bin(s, level, base, past);
-    const int b = same(s.found);
-    base = same(s.found_before);
-    float least = INFINITY, most = -INFINITY;
-    row.template each<4>([&](float l, int index) {
-      if (l >= low && l <= high && bin(l) == b) {
-        least = fminf(least, l);
-        most = fmaxf(most, l);
-        const int at = atomicAdd(&s.listed, 1);
-        if (at < LIST) s.list[at] = entry_of(l, index);
-      }
-    });
-    block_bounds(least, most, s);
-    const int n = same(s.listed);
-    if (n <= LIST) {
-      sort_list(s, n);
-      uint64_t w[EACH], sum = 0, all;
-#pragma unroll
-      for (int i = 0; i < EACH; i++) { const int e = EACH * threadIdx.x + i; w[i] = e < n ? term(entry_logit(s.sorted[e])) : 0; sum += w[i]; }
-      uint64_t before = base + block_before(sum, s, all);
-#pragma unroll
-      for (int i = 0; i < EACH; i++) {
-        if (!past(before) && past(before + w[i])) { s.found = EACH * threadIdx.x + i; s.found_before = before + w[i]; }
-        before += w[i];
-      }
-      __syncthreads();
-      const uint64_t e = same(s.sorted[same(s.found)]);
-      return Found{entry_logit(e), entry_index(e), same(s.found_before)};
-    }
-    if (least == most) {                         // equal ones: the first by index
-      const uint64_t w = term(least);
-      return across(row, s, [&](float l, int) { return l == least ? w : 0; }, Past{past.target, past.reach, base});
-    }
-    low = least;
-    high = most;
-    bin = Bins(low, high);
-    fill_bins(row, s, 1, bin, low, high, term);
-  }
-  return Found{NAN, 0, base};                    // (not reached)
-}
+struct Found {
+  float    logit;
+  int      index;                                // -1: one of several equal ones, whose running sums go on from `before`
+  uint64_t upto, before;                         // the running sums with it and, of equal ones, without any of them
+};
 
 template <class T>
 __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
+  constexpr int N = Row<T>::N;
   __shared__ Shared s;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const int64_t r = blockIdx.x;
   const Row<T> row((const T *)a.logits + r * a.ld, a.vocab);
   const float temperature = a.temperature ? a.temperature[r] : 1.f;
@@ -390,26 +306,32 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
   float top = -INFINITY, low = INFINITY;         // this thread's, then the row's
   if (!(temperature > 0.f)) {
     int first = 0;
-    row.template each<4>([&](float l, int index) { if (l > top) { top = l; first = index; } });
+    row.template each<4>([&](const uint4 &w, int v) {
+#pragma unroll
+      for (int i = 0; i < N; i++) { const float l = Row<T>::logit(w, i); const bool more = l > top; top = more ? l : top; first = more ? row.index(v, i) : first; }
+    });
     // the larger, then the lower index: the largest entry
     uint64_t best = top > -INFINITY ? entry_of(top, first) : 0;
 #pragma unroll
     for (int o = 32; o; o >>= 1) { const uint64_t x = __shfl_xor(best, o); best = x > best ? x : best; }
-    if ((t & 63) == 0) s.part[t >> 6] = best;
+    if (lane == 0) s.part[wave] = best;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WAVES; w++) best = s.part[w] > best ? s.part[w] : best;
     answer(best ? entry_index(best) : 0, best ? 0.f : NAN);
     return;
   }
-  row.template each<4>([&](float l, int) { top = fmaxf(top, l); low = fminf(low, l); });
+  if (t < STEPS) s.steps[t] = exp2((double)t / STEPS);
+  if (t == 0) s.found = 0;
+  row.template each<4>([&](const uint4 &w, int) {
+#pragma unroll
+    for (int i = 0; i < N; i++) { const float l = Row<T>::logit(w, i); top = fmaxf(top, l); low = l > -INFINITY ? fminf(low, l) : low; }
+  });
   const float mine = top;
   block_bounds(low, top, s);
   if (top == -INFINITY) { answer(0, NAN); return; }
-  if (t < STEPS) s.steps[t] = exp2((double)t / STEPS);
-  if (t == 0) s.found = 0;
 
-  const Weight weight{top, STEPS * 1.44269504088896340736 / (double)temperature, s.steps};
+  Weight weight{top, STEPS * 1.44269504088896340736 / (double)temperature, s.steps, false};
   const bool nucleus = p > 0.f && p < 1.f;
   // a weight of at least min_p
   const double drop = least_p > 0.f && temperature < INFINITY ? (double)temperature * log((double)fminf(least_p, 1.f)) : -INFINITY;
@@ -420,115 +342,247 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
   };
   // the number that the walk has to pass: where rounding, or a number of 1, leaves nothing beyond it, the last that weighs something
   auto walk = [&](uint64_t all) { const double target = draw * (double)all; return (double)all > target ? Past{target, false} : Past{(double)all, true}; };
+  auto list = [&](float l, int index) {
+    const int at = atomicAdd(&s.listed, 1);
+    if (at < LIST) s.list[at] = entry_of(l, index);
+  };
 
-  float bound = low;                             // what top_k leaves is not below it
-  if (k > 0 && k < row.V) {
-    if (k <= FEW) {
-      // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
-      float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
-      block_bounds(lowest, dummy, s);
-      const Bins bin(lowest, top, INFINITY);
-      for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
-      __syncthreads();
-      if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
-      if (t == 0) { s.listed = 0; s.found = BINS - 1; }
-      __syncthreads();
-      const bool every = sum_bins(s, 0) < (uint64_t)k;             // fewer maxima than that: all of the row are candidates
-      find_bin(s, 0, 0, Past{(double)k, true});
-      const int last = every ? BINS - 1 : same(s.found);
-      row.template each<4>([&](float l, int index) {
-        if (bin(l) <= last) {
-          const int at = atomicAdd(&s.listed, 1);
-          if (at < LIST) s.list[at] = entry_of(l, index);
+  const bool cut = k > 0 && k < row.V;
+  if (cut && k <= FEW) {
+    // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
+    float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
+    block_bounds(lowest, dummy, s);
+    const Bins bin(lowest, top, INFINITY);
+    for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
+    __syncthreads();
+    if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
+    if (t == 0) { s.listed = 0; s.found = BINS - 1; }
+    __syncthreads();
+    const bool every = sum_bins(s, 0) < (uint64_t)k;               // fewer maxima than that: all of the row are candidates
+    find_bin(s, 0, 0, Past{(double)k, true});
+    const int last = every ? BINS - 1 : same(s.found);
+    row.hits([&](float l) { return bin(l) <= last; }, list);
+    __syncthreads();
+    const int n = same(s.listed);
+    if (n <= LIST) {
+      sort_list(s, n);
+      const uint32_t kth = n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u;
+      uint64_t e[EACH], w[EACH], sum = 0, all;
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        const int at = EACH * t + i;
+        e[i] = at < n ? s.sorted[at] : 0;
+        const uint64_t x = weight(entry_logit(e[i]));
+        w[i] = at < n && (uint32_t)(e[i] >> 32) >= kth ? x : 0;
+        sum += w[i];
+      }
+      uint64_t before = block_before(sum, s, all);
+      const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
+      uint64_t number = 0;
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        const bool stays = !end(before) && enough(entry_logit(e[i]));
+        before += w[i];
+        w[i] = stays ? w[i] : 0;
+        number += w[i] != 0;
+      }
+      if (!nucleus) {                            // by index: the list again with the index first and the place in the order behind it
+        uint64_t at = block_before(number, s, number);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+          if (w[i]) s.list[at++] = (uint64_t)(uint32_t)e[i] << 32 | (uint32_t)(EACH * t + i);
+          s.bins[0][EACH * t + i] = e[i];        // (what was sorted by logit is needed once more)
+          s.bins[1][EACH * t + i] = w[i];
         }
-      });
+        sort_list(s, (int)number);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+          const int j = EACH * t + i;
+          const uint32_t place = j < (int)number ? (uint32_t)s.sorted[j] : 0u;
+          e[i] = s.bins[0][place];
+          w[i] = j < (int)number ? s.bins[1][place] : 0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < EACH; i++) sum += w[i];
+      before = block_before(sum, s, all);
+      const Past past = walk(all);
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        if (!past(before) && past(before + w[i])) s.found_before = e[i];
+        before += w[i];
+      }
       __syncthreads();
+      const uint64_t drawn = same(s.found_before);
+      finish(entry_logit(drawn), entry_index(drawn), all);
+      return;
+    }
+  }
+
+  // Descents, from the largest down: to the k-th largest, to where the nucleus ends, to the token.
+  float bound = low;                             // what top_k leaves is not below it
+  uint64_t all = 0;
+  Past past{0.0, true};
+  Found f{top, 0, 0, 0};
+  enum { KTH, END, TOKEN, NONE };
+  int goal = cut ? KTH : nucleus ? END : NONE;
+  Bins bin(low, top, INFINITY);
+  for (int turn = 0; turn < 3 && goal != NONE; turn++) {
+    float least = bound, most = top;
+    // (a row's own bins and at most three times those of a bin: 2^32 floats are 2^11 times 2^21, 2^10, 1.  Both loops are bounded whatever the sums are, and
+    // every wave takes the same turns: all of them read what decides from the same places between the same two barriers.)
+    uint64_t base = 0, of_enough = 0;
+    for (int level = 0; level < 5; level++) {
+      const int l1 = level ? 1 : 0;
+      if (level || goal != TOKEN) {              // (the token's are those of the nucleus)
+        weight.one = goal == KTH;
+        bin = level ? Bins(least, most) : Bins(bound, top, goal == KTH ? INFINITY : 31.f * temperature);
+        __syncthreads();
+        for (int i = t; i < BINS; i += THREADS) s.bins[l1][i] = 0;
+        __syncthreads();
+        uint64_t sum = 0;
+        row.template each<2>([&](const uint4 &w, int) {
+#pragma unroll
+          for (int i = 0; i < N; i++) {
+            const float l = Row<T>::logit(w, i);
+            if (l >= least && l <= most) {       // (not NaN, and above -infinity like those)
+              const uint64_t x = weight(l);
+              sum += enough(l) ? x : 0;
+              if (x) atomicAdd((unsigned long long *)&s.bins[l1][bin(l)], (unsigned long long)x);
+            }
+          }
+        });
+        __syncthreads();
+        const uint64_t total = sum_bins(s, l1);
+        if (!level) {
+          if (goal == KTH && total <= (uint64_t)k) break;            // nothing to cut: f is the largest, set right below
+          past = Past{goal == KTH ? (double)k : (double)p * (double)total, true};
+          of_enough = block_sum(sum, s);
+        }
+      }
+      __syncthreads();
+      if (t == 0) s.listed = 0;
+      find_bin(s, l1, base, past);
+      const int b = same(s.found);
+      base = same(s.found_before);
+      float lo = INFINITY, hi = -INFINITY;
+      row.hits([&](float l) { return l >= least && l <= most && bin(l) == b; }, [&](float l, int index) {
+        lo = fminf(lo, l);
+        hi = fmaxf(hi, l);
+        list(l, index);
+      });
+      block_bounds(lo, hi, s);
       const int n = same(s.listed);
       if (n <= LIST) {
         sort_list(s, n);
-        const uint32_t kth = n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u;
-        uint64_t e[EACH], w[EACH], sum = 0, all;
+        uint64_t w[EACH], sum = 0, dummy;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          const int at = EACH * t + i;
-          e[i] = at < n ? s.sorted[at] : 0;
-          w[i] = at < n && (uint32_t)(e[i] >> 32) >= kth ? weight(entry_logit(e[i])) : 0;
+          const int e = EACH * t + i;
+          const uint64_t x = weight(entry_logit(e < n ? s.sorted[e] : 0));
+          w[i] = e < n ? x : 0;
           sum += w[i];
         }
-        uint64_t before = block_before(sum, s, all);
-        const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
-        uint64_t number = 0;
+        uint64_t before = base + block_before(sum, s, dummy);
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          const bool stays = !end(before) && enough(entry_logit(e[i]));
-          before += w[i];
-          w[i] = stays ? w[i] : 0;
-          number += w[i] != 0;
-        }
-        if (!nucleus) {                          // by index: the list again with the index first and the place in the order behind it
-          uint64_t at = block_before(number, s, number);
-#pragma unroll
-          for (int i = 0; i < EACH; i++) {
-            if (w[i]) s.list[at++] = (uint64_t)(uint32_t)e[i] << 32 | (uint32_t)(EACH * t + i);
-            s.bins[0][EACH * t + i] = e[i];      // (what was sorted by logit is needed once more)
-          }
-          sort_list(s, (int)number);
-#pragma unroll
-          for (int i = 0; i < EACH; i++) {
-            const int j = EACH * t + i;
-            e[i] = j < (int)number ? s.bins[0][(uint32_t)s.sorted[j]] : 0;
-            w[i] = j < (int)number ? weight(entry_logit(e[i])) : 0;
-          }
-        }
-        sum = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) sum += w[i];
-        before = block_before(sum, s, all);
-        const Past past = walk(all);
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-          if (!past(before) && past(before + w[i])) s.found_before = e[i];
+          if (!past(before) && past(before + w[i])) { s.found = EACH * t + i; s.found_before = before + w[i]; }
           before += w[i];
         }
         __syncthreads();
-        const uint64_t drawn = same(s.found_before);
-        finish(entry_logit(drawn), entry_index(drawn), all);
-        return;
+        const uint64_t e = same(s.sorted[same(s.found)]);
+        f = Found{entry_logit(e), entry_index(e), same(s.found_before), 0};
+        break;
       }
-    }
-    const Bins bin(low, top, INFINITY);
-    const auto one = [](float) { return (uint64_t)1; };
-    if (fill_bins(row, s, 0, bin, low, top, one) > (uint64_t)k) bound = descend(row, s, bin, low, top, one, Past{(double)k, true}).logit;
-  }
-  if (nucleus) {
-    const Bins bin(bound, top, 31.f * temperature);
-    uint64_t sum = 0;
-    const uint64_t of_all = fill_bins(row, s, 0, bin, bound, top, [&](float l) {
-      const uint64_t w = weight(l);
-      if (enough(l)) sum += w;
-      return w;
-    });
-    const uint64_t of_enough = block_sum(sum, s);
-    Past past{(double)p * (double)of_all, true};
-    uint64_t all = 0;
-    Found f;
-    for (int end = 1; end >= 0; end--) {         // where the nucleus ends, then the token
-      f = descend(row, s, bin, bound, top, weight, past);
-      if (end) {
-        all = enough(f.logit) ? f.upto : of_enough;
-        past = walk(all);
+      if (lo == hi) {                            // equal ones: how many of them it takes
+        const uint64_t w = same(weight(lo));
+        uint32_t few = 1, many = (uint32_t)n;
+        for (int i = 0; i < 20 && few < many; i++) {
+          const uint32_t middle = few + (many - few) / 2;
+          if (past(base + middle * w)) many = middle; else few = middle + 1;
+        }
+        f = Found{lo, -1, base + few * w, base};
+        break;
       }
+      least = lo;
+      most = hi;
     }
-    finish(f.logit, f.index, all);
-    return;
+    if (goal == KTH) {
+      bound = past.target > 0.0 ? f.logit : low;
+      past = Past{0.0, true};
+      goal = nucleus ? END : NONE;
+    } else if (goal == END) {
+      all = enough(f.logit) ? f.upto : of_enough;
+      past = walk(all);
+      bin = Bins(bound, top, 31.f * temperature);
+      goal = TOKEN;
+    } else goal = NONE;
   }
-  const auto term = [&](float l, int) { return l >= bound && enough(l) ? weight(l) : 0; };
+  weight.one = false;
+  if (nucleus && f.index >= 0) { finish(f.logit, f.index, all); return; }
+
+  // By index: all that is kept where there is no nucleus, or the equal ones among which the token is.
+  const bool equal = nucleus;
+  const float from = equal ? f.logit : bound, to = equal ? f.logit : top;
+  auto term = [&](float l) {
+    const uint64_t x = weight(l);
+    return l >= from && l <= to && enough(l) ? x : 0;
+  };
+  const int runs = (row.vectors + 63) / 64;
   __syncthreads();
-  uint64_t sum = 0;
-  row.template each<2>([&](float l, int index) { sum += term(l, index); });
-  const uint64_t all = block_sum(sum, s);
-  const Found token = across(row, s, term, walk(all));
-  finish(token.logit, token.index, all);
+  for (int n0 = wave; n0 < runs; n0 += 2 * WAVES) {
+    uint4 w[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) w[j] = row.load((n0 + j * WAVES) * 64 + lane);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float l = Row<T>::logit(w[j], i);
+        if (l >= from && l <= to && enough(l)) sum += weight(l);
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      if (lane == 0 && n0 + j * WAVES < runs) s.runs[n0 + j * WAVES] = sum;
+    }
+  }
+  __syncthreads();
+  const int each = (runs + THREADS - 1) / THREADS, r0 = t * each;
+  uint64_t sum = 0, total;
+  for (int i = 0; i < each; i++) sum += r0 + i < runs ? s.runs[r0 + i] : 0;
+  uint64_t before = block_before(sum, s, total);
+  if (equal) past.base = f.before;
+  else {
+    all = total;
+    past = walk(all);
+  }
+  for (int i = 0; i < each; i++) {
+    const uint64_t x = r0 + i < runs ? s.runs[r0 + i] : 0;
+    if (!past(before) && past(before + x)) { s.found = r0 + i; s.found_before = before; }
+    before += x;
+  }
+  __syncthreads();
+  if (wave == 0) {                               // the run again
+    const int v = same(s.found) * 64 + lane;
+    const uint4 w = row.load(v);
+    uint64_t x[N], mass = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) { x[i] = term(Row<T>::logit(w, i)); mass += x[i]; }
+    uint64_t upto = s.found_before + wave_running(mass) - mass;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const bool here = !past(upto) && past(upto + x[i]);
+      upto += x[i];
+      if (here) {
+        const int token = row.index(v, i);
+        const float l = Row<T>::logit(w, i);
+        a.tokens[r] = token;
+        if (a.logprobs) a.logprobs[r] = (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)all / UNIT));
+      }
+    }
+  }
 }
 
 }  // namespace
