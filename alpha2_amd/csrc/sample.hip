@@ -25,11 +25,13 @@ struct SampleArgs {
   int32_t vocab;
 };
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, BINS = 2048, LIST = 2048, EACH = LIST / THREADS, STEPS = 256;
-static_assert(BINS == LIST, "EACH bins, or entries, to a thread");
+constexpr int BINS = 2048, LIST = 2048, STEPS = 256, MOST_WAVES = 16;
+static_assert(BINS == LIST, "as many bins as entries to a thread");
 constexpr int MAX_VOCAB = 1 << 20;              // sums of as many weights of 2^43 stay below 2^63
 constexpr double UNIT = 0x1p43;
-constexpr int FEW = THREADS / 2;                 // a top_k up to this goes through the threads' maxima, which leave about k candidates
+constexpr int FEW = 256;                         // a top_k up to this goes through the maxima of 512 threads or more, which leave about k candidates
+constexpr int LONG = 16384;                      // rows past this have 1024 threads
+constexpr int SMALL = 512;                       // rows up to this are a list from the start
 
 // f32 -> whole numbers of the same order, -0 as 0; back
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -46,13 +48,13 @@ constexpr int RUNS = MAX_VOCAB / 256 + 1;         // (one more where a row begin
 
 struct Shared {
   uint64_t bins[2][BINS];                        // running sums, of the row's own bins and of a bin's bins
-  uint64_t list[LIST], sorted[LIST];
+  uint64_t list[2][LIST], sorted[LIST];
   uint64_t runs[RUNS];                           // sums of 64 vectors of four (or eight) logits
   double   steps[STEPS];                         // 2^(i / 256)
-  uint64_t part[WAVES];
-  float    low[WAVES], high[WAVES];
-  uint64_t found_before;
-  int      found, listed;
+  uint64_t part[MOST_WAVES];
+  float    low[MOST_WAVES], high[MOST_WAVES];
+  uint64_t found_before, found_entry, answer, kept;
+  int      found, listed[2];
 };
 static_assert(sizeof(Shared) <= 160 * 1024, "a workgroup's LDS");
 
@@ -63,13 +65,26 @@ __device__ __forceinline__ float same(float v) { return __uint_as_float((uint32_
 __device__ __forceinline__ uint64_t same(uint64_t v) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
+// What the lanes hold up to this one, by DPP: a step is two moves and an addition, where __shfl_up is two trips through LDS
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t plus_moved(uint64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ uint64_t wave_running(uint64_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const uint64_t x = __shfl_up(v, o); v += lane >= o ? x : 0; }
-  return v;
+  v = plus_moved<0x111, 0xf>(v);                 // one, two, four, eight to the right in rows of 16
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);                 // the last of a row to the next one, of two rows to the next two
+  return plus_moved<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint64_t wave_last(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 // the sum over the threads before this one, and over all
+template <int THREADS>
 __device__ __forceinline__ uint64_t block_before(uint64_t v, Shared &s, uint64_t &all) {
   const int wave = threadIdx.x >> 6;
   const uint64_t upto = wave_running(v);
@@ -79,21 +94,17 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, Shared &s, uint64_t
   uint64_t before = 0;
   all = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; w++) { const uint64_t x = s.part[w]; all += x; before += w < wave ? x : 0; }
+  for (int w = 0; w < THREADS / 64; w++) { const uint64_t x = s.part[w]; all += x; before += w < wave ? x : 0; }
   all = same(all);
   return before + upto - v;
 }
+template <int THREADS>
 __device__ __forceinline__ uint64_t block_sum(uint64_t v, Shared &s) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  uint64_t all = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; w++) all += s.part[w];
-  return same(all);
+  uint64_t all;
+  block_before<THREADS>(v, s, all);
+  return all;
 }
+template <int THREADS>
 __device__ __forceinline__ void block_bounds(float &low, float &high, Shared &s) {
   low = -wave_max(-low);
   high = wave_max(high);
@@ -101,29 +112,31 @@ __device__ __forceinline__ void block_bounds(float &low, float &high, Shared &s)
   if ((threadIdx.x & 63) == 0) { s.low[threadIdx.x >> 6] = low; s.high[threadIdx.x >> 6] = high; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WAVES; w++) { low = fminf(low, s.low[w]); high = fmaxf(high, s.high[w]); }
+  for (int w = 0; w < THREADS / 64; w++) { low = fminf(low, s.low[w]); high = fmaxf(high, s.high[w]); }
   low = same(low);
   high = same(high);
 }
 
-// The first n entries of `list` in order, into `sorted`.  Up to 256 by counting the larger ones of each, 2 to 8 threads to an entry; more by exchanges,
+// The n entries of a list in order, into `sorted`.  Up to 256 by counting the larger ones of each, 2 to 16 threads to an entry; more by exchanges,
 // whose steps between neighbours of 128 need no barrier.
-__device__ __forceinline__ void sort_list(Shared &s, int n) {
+template <int THREADS>
+__device__ __forceinline__ void sort_list(Shared &s, const uint64_t *list, int n) {
   const int t = threadIdx.x;
   __syncthreads();
-  if (n <= THREADS / 2) {
-    const int shift = n <= THREADS / 8 ? 3 : n <= THREADS / 4 ? 2 : 1, i = t >> shift;
-    const uint64_t mine = i < n ? s.list[i] : 0;
+  if (n <= 256) {
+    const int most = THREADS == 512 ? 3 : 4, shift = n <= 64 ? most : n <= 128 ? most - 1 : most - 2, i = t >> shift;
+    const uint64_t mine = i < n ? list[i] : 0;
     uint32_t larger = 0;
-    for (int j = t & ((1 << shift) - 1); j < n; j += 1 << shift) larger += s.list[j] > mine;
+    for (int j = t & ((1 << shift) - 1); j < n; j += 1 << shift) larger += list[j] > mine;
     larger += lane_xor<1>(larger);
     if (shift > 1) larger += lane_xor<2>(larger);
     if (shift > 2) larger += lane_xor<4>(larger);
+    if (shift > 3) larger += lane_xor<8>(larger);
     if (i < n && (t & ((1 << shift) - 1)) == 0) s.sorted[larger] = mine;
   } else {
-    int size = THREADS;
+    int size = 512;
     while (size < n) size <<= 1;
-    for (int i = t; i < size; i += THREADS) s.sorted[i] = i < n ? s.list[i] : 0;
+    for (int i = t; i < size; i += THREADS) s.sorted[i] = i < n ? list[i] : 0;
     __syncthreads();
     for (int run = 2; run <= size; run <<= 1)
       for (int apart = run >> 1; apart; apart >>= 1) {
@@ -147,37 +160,28 @@ struct Past {                                    // a running sum, on from `base
   __device__ __forceinline__ bool operator()(uint64_t s) const { const double x = (double)(base + s); return reach ? x >= target : x > target; }
 };
 
-template <class T> struct Row {
+template <class T, int THREADS> struct Row {
   static constexpr int N = 16 / sizeof(T);       // logits to a vector
-  const T *x;                                    // of the first vector, at or before the row's first logit
-  int lead, V, vectors;
+  // The logits before the first whole 16 bytes and behind the last are vectors of one each, so that no other memory is read; all are in the order of the indices.
+  const T *x;
+  int V, head, whole, vectors;
   __device__ __forceinline__ Row(const T *row, int vocab) {
-    lead = (int)((uintptr_t)row % 16 / sizeof(T));
-    x = row - lead;
+    x = row;
     V = vocab;
-    vectors = (lead + V + N - 1) / N;
+    head = min((int)((16 - (uintptr_t)row % 16) % 16 / sizeof(T)), V);
+    whole = (V - head) / N;
+    vectors = V - whole * (N - 1);
   }
-  __device__ __forceinline__ int index(int v, int i) const { return v * N + i - lead; }
-  __device__ __forceinline__ float at(int index) const { return Io<T>::ld(x, (size_t)(index + lead)); }
-  // vector v as it is stored; what is not the row's is not read, and NaN
+  __device__ __forceinline__ int index(int v, int i) const {
+    const int n = v - head;
+    return v < head ? v : n < whole ? head + n * N + i : v + whole * (N - 1);
+  }
+  __device__ __forceinline__ float at(int index) const { return Io<T>::ld(x, (size_t)index); }
+  // vector v as it is stored; NaN where there is no logit
   __device__ __forceinline__ uint4 load(int v) const {
     uint4 w = make_uint4(~0u, ~0u, ~0u, ~0u);
-    if (v > 0 && v < vectors - 1) w = *reinterpret_cast<const uint4 *>(x + (int64_t)v * N);
-    else if (v < vectors) {
-      uint32_t u[4] = {~0u, ~0u, ~0u, ~0u};
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        const bool in = index(v, i) >= 0 && index(v, i) < V;
-        if (in) {
-          if constexpr (N == 4) u[i] = __float_as_uint(at(index(v, i)));
-          else {
-            const uint32_t half = __float_as_uint(at(index(v, i))) >> 16;
-            u[i / 2] = i & 1 ? (u[i / 2] & 0xffffu) | half << 16 : (u[i / 2] & 0xffff0000u) | half;
-          }
-        }
-      }
-      w = make_uint4(u[0], u[1], u[2], u[3]);
-    }
+    if (v >= head && v - head < whole) w = *reinterpret_cast<const uint4 *>(x + head + (int64_t)(v - head) * N);
+    else if (v < vectors) w.x = N == 4 ? __float_as_uint(at(index(v, 0))) : __float_as_uint(at(index(v, 0))) >> 16 | 0xffff0000u;
     return w;
   }
   static __device__ __forceinline__ float logit(const uint4 &w, int i) {
@@ -198,7 +202,7 @@ template <class T> struct Row {
   // f(logit, index) for the ones above -infinity for which `hit` holds, which are few: the loop over them is there once
   template <class Hit, class F>
   __device__ __forceinline__ void hits(Hit hit, F f) const {
-    constexpr int U = 4;
+    constexpr int U = 16 / N;                    // (16 tests written out)
     for (int v0 = threadIdx.x; v0 < vectors; v0 += THREADS * U) {
       uint4 w[U];
 #pragma unroll
@@ -259,27 +263,37 @@ struct Bins {
     const float at = (high - l) * scale;
     return at < (float)(BINS - 1) ? (int)at : BINS - 1;       // (0 x infinity: the last)
   }
+  // the same, asked of one bin
+  __device__ __forceinline__ bool in(float l, int b) const {
+    if (shift >= 0) return (int)((order_of(high) - order_of(l)) >> shift) == b;
+    const float at = (high - l) * scale;
+    return b < BINS - 1 ? at >= (float)b && at < (float)(b + 1) : !(at < (float)(BINS - 1));
+  }
 };
 static_assert(BINS == 1 << 11, "the shift of a bin's bins");
 
 // s.bins[level] to running sums; the sum of all
+template <int THREADS>
 __device__ __forceinline__ uint64_t sum_bins(Shared &s, int level) {
+  constexpr int EACH = BINS / THREADS;
   uint64_t x[EACH], sum = 0, all;
 #pragma unroll
   for (int i = 0; i < EACH; i++) { x[i] = s.bins[level][EACH * threadIdx.x + i]; sum += x[i]; }
-  uint64_t upto = block_before(sum, s, all);
+  uint64_t upto = block_before<THREADS>(sum, s, all);
 #pragma unroll
   for (int i = 0; i < EACH; i++) { upto += x[i]; s.bins[level][EACH * threadIdx.x + i] = upto; }
   __syncthreads();
   return all;
 }
-// Where in s.bins[level] a running sum, on from `base`, passes: the bin into s.found, the sum before it into s.found_before.
+// Where in s.bins[level] running sums, on from `base`, pass: the bin into s.found, the sum before it into s.found_before.
+template <int THREADS>
 __device__ __forceinline__ void find_bin(Shared &s, int level, uint64_t base, const Past &past) {
+  constexpr int EACH = BINS / THREADS;
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
     const int b = EACH * threadIdx.x + i;
-    const uint64_t before = base + (b ? s.bins[level][b - 1] : 0);
-    if (!past(before) && past(base + s.bins[level][b])) { s.found = b; s.found_before = before; }
+    const uint64_t before = base + (b ? s.bins[level][b - 1] : 0), upto = base + s.bins[level][b];
+    if (!past(before) && past(upto)) { s.found = b; s.found_before = before; }
   }
   __syncthreads();
 }
@@ -290,25 +304,24 @@ struct Found {
   uint64_t upto, before;                         // the running sums with it and, of equal ones, without any of them
 };
 
-template <class T>
+template <class T, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
-  constexpr int N = Row<T>::N;
+  constexpr int WAVES = THREADS / 64, EACH = LIST / THREADS, N = Row<T, THREADS>::N;
   __shared__ Shared s;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const int64_t r = blockIdx.x;
-  const Row<T> row((const T *)a.logits + r * a.ld, a.vocab);
+  const Row<T, THREADS> row((const T *)a.logits + r * a.ld, a.vocab);
+  auto logit = [](const uint4 &w, int i) { return Row<T, THREADS>::logit(w, i); };
   const float temperature = a.temperature ? a.temperature[r] : 1.f;
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 0.f, least_p = a.min_p ? a.min_p[r] : 0.f, u = a.uniform[r];
-  auto answer = [&](int token, float logprob) {
-    if (t == 0) { a.tokens[r] = token; if (a.logprobs) a.logprobs[r] = logprob; }
-  };
+  auto answer = [&](int token, float logprob) { a.tokens[r] = token; if (a.logprobs) a.logprobs[r] = logprob; };      // by one thread
   float top = -INFINITY, low = INFINITY;         // this thread's, then the row's
   if (!(temperature > 0.f)) {
     int first = 0;
     row.template each<4>([&](const uint4 &w, int v) {
 #pragma unroll
-      for (int i = 0; i < N; i++) { const float l = Row<T>::logit(w, i); const bool more = l > top; top = more ? l : top; first = more ? row.index(v, i) : first; }
+      for (int i = 0; i < N; i++) { const float l = logit(w, i); const bool more = l > top; top = more ? l : top; first = more ? row.index(v, i) : first; }
     });
     // the larger, then the lower index: the largest entry
     uint64_t best = top > -INFINITY ? entry_of(top, first) : 0;
@@ -318,270 +331,325 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WAVES; w++) best = s.part[w] > best ? s.part[w] : best;
-    answer(best ? entry_index(best) : 0, best ? 0.f : NAN);
+    if (t == 0) answer(best ? entry_index(best) : 0, best ? 0.f : NAN);
     return;
   }
   if (t < STEPS) s.steps[t] = exp2((double)t / STEPS);
-  if (t == 0) s.found = 0;
+  if (t == 0) { s.found = 0; s.listed[0] = s.listed[1] = 0; s.answer = 0; s.kept = 0; }
   row.template each<4>([&](const uint4 &w, int) {
 #pragma unroll
-    for (int i = 0; i < N; i++) { const float l = Row<T>::logit(w, i); top = fmaxf(top, l); low = l > -INFINITY ? fminf(low, l) : low; }
+    for (int i = 0; i < N; i++) { const float l = logit(w, i); top = fmaxf(top, l); low = l > -INFINITY ? fminf(low, l) : low; }
   });
   const float mine = top;
-  block_bounds(low, top, s);
-  if (top == -INFINITY) { answer(0, NAN); return; }
+  block_bounds<THREADS>(low, top, s);
+  if (top == -INFINITY) { if (t == 0) answer(0, NAN); return; }
 
   Weight weight{top, STEPS * 1.44269504088896340736 / (double)temperature, s.steps, false};
-  const bool nucleus = p > 0.f && p < 1.f;
+  const bool nucleus = p > 0.f && p < 1.f, cut = k > 0 && k < row.V;
   // a weight of at least min_p
   const double drop = least_p > 0.f && temperature < INFINITY ? (double)temperature * log((double)fminf(least_p, 1.f)) : -INFINITY;
   auto enough = [&](float l) { return l == top || (double)l - (double)top >= drop; };
   const double draw = fmin(fmax((double)u, 0.0), 1.0);
-  auto finish = [&](float l, int token, uint64_t all) {
-    answer(token, (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)all / UNIT)));
-  };
+  // what one thread finds: the token and the sum of what is kept
+  auto finish = [&](uint64_t entry, uint64_t all) { s.answer = entry; s.kept = all; };
   // the number that the walk has to pass: where rounding, or a number of 1, leaves nothing beyond it, the last that weighs something
   auto walk = [&](uint64_t all) { const double target = draw * (double)all; return (double)all > target ? Past{target, false} : Past{(double)all, true}; };
-  auto list = [&](float l, int index) {
-    const int at = atomicAdd(&s.listed, 1);
-    if (at < LIST) s.list[at] = entry_of(l, index);
+  auto list = [&](int which, float l, int index) {
+    const int at = atomicAdd(&s.listed[which], 1);
+    if (at < LIST) s.list[which][at] = entry_of(l, index);
   };
 
-  const bool cut = k > 0 && k < row.V;
-  if (cut && k <= FEW) {
-    // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
-    float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
-    block_bounds(lowest, dummy, s);
-    const Bins bin(lowest, top, INFINITY);
-    for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
-    __syncthreads();
-    if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
-    if (t == 0) { s.listed = 0; s.found = BINS - 1; }
-    __syncthreads();
-    const bool every = sum_bins(s, 0) < (uint64_t)k;               // fewer maxima than that: all of the row are candidates
-    find_bin(s, 0, 0, Past{(double)k, true});
-    const int last = every ? BINS - 1 : same(s.found);
-    row.hits([&](float l) { return bin(l) <= last; }, list);
-    __syncthreads();
-    const int n = same(s.listed);
-    if (n <= LIST) {
-      sort_list(s, n);
-      const uint32_t kth = n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u;
-      uint64_t e[EACH], w[EACH], sum = 0, all;
-#pragma unroll
-      for (int i = 0; i < EACH; i++) {
-        const int at = EACH * t + i;
-        e[i] = at < n ? s.sorted[at] : 0;
-        const uint64_t x = weight(entry_logit(e[i]));
-        w[i] = at < n && (uint32_t)(e[i] >> 32) >= kth ? x : 0;
-        sum += w[i];
-      }
-      uint64_t before = block_before(sum, s, all);
-      const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
-      uint64_t number = 0;
-      sum = 0;
-#pragma unroll
-      for (int i = 0; i < EACH; i++) {
-        const bool stays = !end(before) && enough(entry_logit(e[i]));
-        before += w[i];
-        w[i] = stays ? w[i] : 0;
-        number += w[i] != 0;
-      }
-      if (!nucleus) {                            // by index: the list again with the index first and the place in the order behind it
-        uint64_t at = block_before(number, s, number);
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-          if (w[i]) s.list[at++] = (uint64_t)(uint32_t)e[i] << 32 | (uint32_t)(EACH * t + i);
-          s.bins[0][EACH * t + i] = e[i];        // (what was sorted by logit is needed once more)
-          s.bins[1][EACH * t + i] = w[i];
-        }
-        sort_list(s, (int)number);
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-          const int j = EACH * t + i;
-          const uint32_t place = j < (int)number ? (uint32_t)s.sorted[j] : 0u;
-          e[i] = s.bins[0][place];
-          w[i] = j < (int)number ? s.bins[1][place] : 0;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < EACH; i++) sum += w[i];
-      before = block_before(sum, s, all);
-      const Past past = walk(all);
-#pragma unroll
-      for (int i = 0; i < EACH; i++) {
-        if (!past(before) && past(before + w[i])) s.found_before = e[i];
-        before += w[i];
+  auto choose = [&] {
+    const bool small = row.V <= SMALL;
+    if (small || (cut && k <= FEW)) {
+      if (small) row.hits([](float) { return true; }, [&](float l, int index) { list(0, l, index); });
+      else {
+        // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
+        float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
+        block_bounds<THREADS>(lowest, dummy, s);
+        const Bins bin(lowest, top, INFINITY);
+        for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
+        __syncthreads();
+        if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
+        __syncthreads();
+        const bool every = sum_bins<THREADS>(s, 0) < (uint64_t)k;    // fewer maxima than that: all of the row are candidates
+        find_bin<THREADS>(s, 0, 0, Past{(double)k, true});
+        const float to = every ? INFINITY : (float)(same(s.found) + 1);        // (the last bin has no end)
+        row.hits([&](float l) { return (bin.high - l) * bin.scale < to || to >= (float)BINS; }, [&](float l, int index) { list(0, l, index); });
       }
       __syncthreads();
-      const uint64_t drawn = same(s.found_before);
-      finish(entry_logit(drawn), entry_index(drawn), all);
-      return;
-    }
-  }
-
-  // Descents, from the largest down: to the k-th largest, to where the nucleus ends, to the token.
-  float bound = low;                             // what top_k leaves is not below it
-  uint64_t all = 0;
-  Past past{0.0, true};
-  Found f{top, 0, 0, 0};
-  enum { KTH, END, TOKEN, NONE };
-  int goal = cut ? KTH : nucleus ? END : NONE;
-  Bins bin(low, top, INFINITY);
-  for (int turn = 0; turn < 3 && goal != NONE; turn++) {
-    float least = bound, most = top;
-    // (a row's own bins and at most three times those of a bin: 2^32 floats are 2^11 times 2^21, 2^10, 1.  Both loops are bounded whatever the sums are, and
-    // every wave takes the same turns: all of them read what decides from the same places between the same two barriers.)
-    uint64_t base = 0, of_enough = 0;
-    for (int level = 0; level < 5; level++) {
-      const int l1 = level ? 1 : 0;
-      if (level || goal != TOKEN) {              // (the token's are those of the nucleus)
-        weight.one = goal == KTH;
-        bin = level ? Bins(least, most) : Bins(bound, top, goal == KTH ? INFINITY : 31.f * temperature);
-        __syncthreads();
-        for (int i = t; i < BINS; i += THREADS) s.bins[l1][i] = 0;
-        __syncthreads();
-        uint64_t sum = 0;
-        row.template each<2>([&](const uint4 &w, int) {
-#pragma unroll
-          for (int i = 0; i < N; i++) {
-            const float l = Row<T>::logit(w, i);
-            if (l >= least && l <= most) {       // (not NaN, and above -infinity like those)
-              const uint64_t x = weight(l);
-              sum += enough(l) ? x : 0;
-              if (x) atomicAdd((unsigned long long *)&s.bins[l1][bin(l)], (unsigned long long)x);
-            }
-          }
-        });
-        __syncthreads();
-        const uint64_t total = sum_bins(s, l1);
-        if (!level) {
-          if (goal == KTH && total <= (uint64_t)k) break;            // nothing to cut: f is the largest, set right below
-          past = Past{goal == KTH ? (double)k : (double)p * (double)total, true};
-          of_enough = block_sum(sum, s);
-        }
-      }
-      __syncthreads();
-      if (t == 0) s.listed = 0;
-      find_bin(s, l1, base, past);
-      const int b = same(s.found);
-      base = same(s.found_before);
-      float lo = INFINITY, hi = -INFINITY;
-      row.hits([&](float l) { return l >= least && l <= most && bin(l) == b; }, [&](float l, int index) {
-        lo = fminf(lo, l);
-        hi = fmaxf(hi, l);
-        list(l, index);
-      });
-      block_bounds(lo, hi, s);
-      const int n = same(s.listed);
+      const int n = same(s.listed[0]);
       if (n <= LIST) {
-        sort_list(s, n);
-        uint64_t w[EACH], sum = 0, dummy;
+        sort_list<THREADS>(s, s.list[0], n);
+        const uint32_t kth = cut && n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u;
+        if (n <= 64) {                             // a wave alone
+          if (wave) return;
+          const uint64_t e = lane < n ? s.sorted[lane] : 0;
+          const float l = entry_logit(e);
+          const uint64_t x = weight(l);
+          uint64_t w = lane < n && (uint32_t)(e >> 32) >= kth ? x : 0, upto = wave_running(w), all = wave_last(upto);
+          const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
+          w = !end(upto - w) && enough(l) ? w : 0;
+          upto = wave_running(w);
+          all = wave_last(upto);
+          if (!nucleus) {                          // by index
+            s.bins[0][lane] = (uint32_t)e;
+            s.bins[1][lane] = w;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            upto = 0;
+            for (int j = 0; j < n; j++) { const uint64_t other = s.bins[0][j], more = s.bins[1][j]; upto += other >= (uint32_t)e ? more : 0; }
+          }
+          const Past past = walk(all);
+          if (!past(upto - w) && past(upto)) finish(e, all);
+          return;
+        }
+        uint64_t e[EACH], w[EACH], sum = 0, all;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          const int e = EACH * t + i;
-          const uint64_t x = weight(entry_logit(e < n ? s.sorted[e] : 0));
-          w[i] = e < n ? x : 0;
+          const int at = EACH * t + i;
+          e[i] = at < n ? s.sorted[at] : 0;
+          const uint64_t x = weight(entry_logit(e[i]));
+          w[i] = at < n && (uint32_t)(e[i] >> 32) >= kth ? x : 0;
           sum += w[i];
         }
-        uint64_t before = base + block_before(sum, s, dummy);
+        uint64_t before = block_before<THREADS>(sum, s, all);
+        const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
+        uint64_t number = 0;
+        sum = 0;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          if (!past(before) && past(before + w[i])) { s.found = EACH * t + i; s.found_before = before + w[i]; }
+          const bool stays = !end(before) && enough(entry_logit(e[i]));
+          before += w[i];
+          w[i] = stays ? w[i] : 0;
+          number += w[i] != 0;
+        }
+        if (!nucleus) {                            // by index: the list again with the index first and the place in the order behind it
+          uint64_t at = block_before<THREADS>(number, s, number);
+#pragma unroll
+          for (int i = 0; i < EACH; i++) {
+            if (w[i]) s.list[0][at++] = (uint64_t)(uint32_t)e[i] << 32 | (uint32_t)(EACH * t + i);
+            s.bins[0][EACH * t + i] = e[i];        // (what was sorted by logit is needed once more)
+            s.bins[1][EACH * t + i] = w[i];
+          }
+          sort_list<THREADS>(s, s.list[0], (int)number);
+#pragma unroll
+          for (int i = 0; i < EACH; i++) {
+            const int j = EACH * t + i;
+            const uint32_t place = j < (int)number ? (uint32_t)s.sorted[j] : 0u;
+            e[i] = s.bins[0][place];
+            w[i] = j < (int)number ? s.bins[1][place] : 0;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) sum += w[i];
+        before = block_before<THREADS>(sum, s, all);
+        const Past past = walk(all);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+          if (!past(before) && past(before + w[i])) finish(e[i], all);
           before += w[i];
         }
-        __syncthreads();
-        const uint64_t e = same(s.sorted[same(s.found)]);
-        f = Found{entry_logit(e), entry_index(e), same(s.found_before), 0};
-        break;
+        return;
       }
-      if (lo == hi) {                            // equal ones: how many of them it takes
-        const uint64_t w = same(weight(lo));
-        uint32_t few = 1, many = (uint32_t)n;
-        for (int i = 0; i < 20 && few < many; i++) {
-          const uint32_t middle = few + (many - few) / 2;
-          if (past(base + middle * w)) many = middle; else few = middle + 1;
-        }
-        f = Found{lo, -1, base + few * w, base};
-        break;
-      }
-      least = lo;
-      most = hi;
     }
-    if (goal == KTH) {
-      bound = past.target > 0.0 ? f.logit : low;
-      past = Past{0.0, true};
-      goal = nucleus ? END : NONE;
-    } else if (goal == END) {
-      all = enough(f.logit) ? f.upto : of_enough;
-      past = walk(all);
-      bin = Bins(bound, top, 31.f * temperature);
-      goal = TOKEN;
-    } else goal = NONE;
-  }
-  weight.one = false;
-  if (nucleus && f.index >= 0) { finish(f.logit, f.index, all); return; }
 
-  // By index: all that is kept where there is no nucleus, or the equal ones among which the token is.
-  const bool equal = nucleus;
-  const float from = equal ? f.logit : bound, to = equal ? f.logit : top;
-  auto term = [&](float l) {
-    const uint64_t x = weight(l);
-    return l >= from && l <= to && enough(l) ? x : 0;
-  };
-  const int runs = (row.vectors + 63) / 64;
-  __syncthreads();
-  for (int n0 = wave; n0 < runs; n0 += 2 * WAVES) {
-    uint4 w[2];
+    // Descents, from the largest down: to the k-th largest, to where the nucleus ends, to the token.
+    float bound = low;                             // what top_k leaves is not below it
+    uint64_t all = 0;
+    Past past{0.0, true};
+    Found f{top, 0, 0, 0};
+    enum { KTH, END, TOKEN, NONE };
+    int goal = cut ? KTH : nucleus ? END : NONE;
+    Bins bin(low, top, INFINITY);
+    // The row's own bins whose members are in the two lists: the one the nucleus ends in and, so that the row need not be gone over again, the one the
+    // token is in if it ends with that bin.
+    int have[2] = {-1, -1}, members[2] = {0, 0};
+    for (int turn = 0; turn < 3 && goal != NONE; turn++) {
+      float least = bound, most = top;
+      // (a row's own bins and at most three times those of a bin: 2^32 floats are 2^11 times 2^21, 2^10, 1.  Both loops are bounded whatever the sums are, and
+      // every wave takes the same turns: all of them read what decides from the same places between the same two barriers.)
+      uint64_t base = 0, of_enough = 0;
+      for (int level = 0; level < 5; level++) {
+        const int l1 = level ? 1 : 0;
+        if (level || goal != TOKEN) {              // (the token's are those of the nucleus)
+          weight.one = goal == KTH;
+          bin = level ? Bins(least, most) : Bins(bound, top, goal == KTH ? INFINITY : 31.f * temperature);
+          __syncthreads();
+          for (int i = t; i < BINS; i += THREADS) s.bins[l1][i] = 0;
+          __syncthreads();
+          uint64_t sum = 0;
+          row.template each<8 / N>([&](const uint4 &w, int) {
 #pragma unroll
-    for (int j = 0; j < 2; j++) w[j] = row.load((n0 + j * WAVES) * 64 + lane);
+            for (int i = 0; i < N; i++) {
+              const float l = logit(w, i);
+              if (l >= least && l <= most) {       // (not NaN, and above -infinity like those)
+                const uint64_t x = weight(l);
+                sum += enough(l) ? x : 0;
+                if (x) atomicAdd((unsigned long long *)&s.bins[l1][bin(l)], (unsigned long long)x);
+              }
+            }
+          });
+          __syncthreads();
+          const uint64_t total = sum_bins<THREADS>(s, l1);
+          if (!level) {
+            if (goal == KTH && total <= (uint64_t)k) break;            // nothing to cut
+            past = Past{goal == KTH ? (double)k : (double)p * (double)total, true};
+            if (goal == END) of_enough = block_sum<THREADS>(sum, s);
+          }
+        }
+        __syncthreads();
+        if (t == 0 && (level || goal != TOKEN)) s.listed[0] = s.listed[1] = 0;
+        find_bin<THREADS>(s, l1, base, past);
+        const int b = same(s.found);
+        base = same(s.found_before);
+        int which = 0, n = 0;
+        const bool listed = !level && goal == TOKEN && (b == have[0] || b == have[1]);
+        if (listed) {
+          which = b == have[0] ? 0 : 1;
+          n = members[which];
+        } else {
+          int too = -1;
+          if (!level && goal == END) {
+            const Past then = walk(same(s.bins[0][b]));
+            __syncthreads();
+            find_bin<THREADS>(s, 0, 0, then);
+            too = same(s.found);
+          } else if (!level && goal == TOKEN) {    // (neither list: the first is made anew)
+            __syncthreads();
+            if (t == 0) s.listed[0] = 0;
+            __syncthreads();
+          }
+          row.hits([&](float l) { return l >= least && l <= most && (bin.in(l, b) || (too >= 0 && bin.in(l, too))); },
+                   [&](float l, int index) { list(bin.in(l, b) ? 0 : 1, l, index); });
+          __syncthreads();
+          n = same(s.listed[0]);
+          if (!level && goal == END) {
+            have[0] = b;
+            members[0] = n;
+            have[1] = too == b ? -1 : too;
+            members[1] = same(s.listed[1]);
+          } else if (goal == END) have[0] = -1;
+        }
+        if (n <= LIST) {
+          if (!(listed && which == 0)) sort_list<THREADS>(s, s.list[which], n);        // (the nucleus's is sorted)
+          uint64_t w[EACH], sum = 0, dummy;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      uint64_t sum = 0;
+          for (int i = 0; i < EACH; i++) {
+            const int e = EACH * t + i;
+            const uint64_t x = weight(entry_logit(e < n ? s.sorted[e] : 0));
+            w[i] = e < n ? x : 0;
+            sum += w[i];
+          }
+          uint64_t before = base + block_before<THREADS>(sum, s, dummy);
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        const float l = Row<T>::logit(w[j], i);
-        if (l >= from && l <= to && enough(l)) sum += weight(l);
+          for (int i = 0; i < EACH; i++) {
+            if (!past(before) && past(before + w[i])) {
+              const uint64_t e = s.sorted[EACH * t + i];
+              if (goal == TOKEN) finish(e, all);
+              else { s.found_entry = e; s.found_before = before + w[i]; }
+            }
+            before += w[i];
+          }
+          if (goal == TOKEN) return;
+          __syncthreads();
+          const uint64_t e = same(s.found_entry);
+          f = Found{entry_logit(e), entry_index(e), same(s.found_before), 0};
+          break;
+        }
+        float lo = INFINITY, hi = -INFINITY;
+        row.hits([&](float l) { return l >= least && l <= most && bin.in(l, b); }, [&](float l, int) { lo = fminf(lo, l); hi = fmaxf(hi, l); });
+        block_bounds<THREADS>(lo, hi, s);
+        if (lo == hi) {                            // equal ones: how many of them it takes
+          const uint64_t w = same(weight(lo));
+          uint32_t few = 1, many = (uint32_t)n;
+          for (int i = 0; i < 20 && few < many; i++) {
+            const uint32_t middle = few + (many - few) / 2;
+            if (past(base + middle * w)) many = middle; else few = middle + 1;
+          }
+          f = Found{lo, -1, base + few * w, base};
+          break;
+        }
+        least = lo;
+        most = hi;
       }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-      if (lane == 0 && n0 + j * WAVES < runs) s.runs[n0 + j * WAVES] = sum;
+      if (goal == KTH) {
+        bound = past.target > 0.0 ? f.logit : low;
+        past = Past{0.0, true};
+        goal = nucleus ? END : NONE;
+      } else if (goal == END) {
+        all = enough(f.logit) ? f.upto : of_enough;
+        past = walk(all);
+        bin = Bins(bound, top, 31.f * temperature);
+        goal = TOKEN;
+      } else goal = NONE;
     }
-  }
-  __syncthreads();
-  const int each = (runs + THREADS - 1) / THREADS, r0 = t * each;
-  uint64_t sum = 0, total;
-  for (int i = 0; i < each; i++) sum += r0 + i < runs ? s.runs[r0 + i] : 0;
-  uint64_t before = block_before(sum, s, total);
-  if (equal) past.base = f.before;
-  else {
-    all = total;
-    past = walk(all);
-  }
-  for (int i = 0; i < each; i++) {
-    const uint64_t x = r0 + i < runs ? s.runs[r0 + i] : 0;
-    if (!past(before) && past(before + x)) { s.found = r0 + i; s.found_before = before; }
-    before += x;
-  }
-  __syncthreads();
-  if (wave == 0) {                               // the run again
-    const int v = same(s.found) * 64 + lane;
+    weight.one = false;
+
+    // By index: all that is kept where there is no nucleus, or the equal ones among which the token is.
+    const bool equal = nucleus;
+    const float from = equal ? f.logit : bound, to = equal ? f.logit : top;
+    const int runs = (row.vectors + 63) / 64;
+    __syncthreads();
+    for (int n0 = wave; n0 < runs; n0 += 2 * WAVES) {
+      uint4 w[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) w[j] = row.load((n0 + j * WAVES) * 64 + lane);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          const float l = logit(w[j], i);
+          if (l >= from && l <= to && enough(l)) sum += weight(l);
+        }
+        sum = wave_running(sum);
+        if (lane == 63 && n0 + j * WAVES < runs) s.runs[n0 + j * WAVES] = sum;
+      }
+    }
+    __syncthreads();
+    const int each = (runs + THREADS - 1) / THREADS, r0 = t * each;
+    uint64_t sum = 0, total;
+    for (int i = 0; i < each; i++) sum += r0 + i < runs ? s.runs[r0 + i] : 0;
+    uint64_t before = block_before<THREADS>(sum, s, total);
+    if (equal) past.base = f.before;
+    else {
+      all = total;
+      past = walk(all);
+    }
+    for (int i = 0; i < each; i++) {
+      const uint64_t x = r0 + i < runs ? s.runs[r0 + i] : 0;
+      if (!past(before) && past(before + x)) { s.found = r0 + i; s.found_before = before; }
+      before += x;
+    }
+    __syncthreads();
+    if (wave) return;
+    const int v = same(s.found) * 64 + lane;       // the run again
     const uint4 w = row.load(v);
     uint64_t x[N], mass = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) { x[i] = term(Row<T>::logit(w, i)); mass += x[i]; }
+    for (int i = 0; i < N; i++) {
+      const float l = logit(w, i);
+      const uint64_t y = weight(l);
+      x[i] = l >= from && l <= to && enough(l) ? y : 0;
+      mass += x[i];
+    }
     uint64_t upto = s.found_before + wave_running(mass) - mass;
+    int token = -1;
+    float l = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const bool here = !past(upto) && past(upto + x[i]);
       upto += x[i];
-      if (here) {
-        const int token = row.index(v, i);
-        const float l = Row<T>::logit(w, i);
-        a.tokens[r] = token;
-        if (a.logprobs) a.logprobs[r] = (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)all / UNIT));
-      }
+      token = here ? row.index(v, i) : token;
+      l = here ? logit(w, i) : l;
     }
+    if (token >= 0) finish(entry_of(l, token), all);
+  };
+  choose();
+  __syncthreads();
+  if (t == 0) {
+    const float l = entry_logit(s.answer);
+    answer(entry_index(s.answer), (float)((l == top ? 0.0 : ((double)l - (double)top) / (double)temperature) - log((double)s.kept / UNIT)));
   }
 }
 
@@ -599,7 +667,8 @@ extern "C" int32_t ah_sample(const AhSample *d) {
   if (d->rows == 0) return AH_OK;
   const SampleArgs a{dp<void>(d->logits), dp<float>(d->temperature), dp<float>(d->top_p), dp<float>(d->min_p), dp<float>(d->uniform), dp<int32_t>(d->top_k),
                      dp<int32_t>(d->tokens), dp<float>(d->logprobs), d->ld, d->vocab};
-  launch_kernel(d->dtype == AH_F32 ? k_sample<float> : k_sample<uint16_t>, dim3((unsigned)d->rows), dim3(THREADS), 0, a);
+  if (d->vocab > LONG) launch_kernel(d->dtype == AH_F32 ? k_sample<float, 1024> : k_sample<uint16_t, 1024>, dim3((unsigned)d->rows), dim3(1024), 0, a);
+  else launch_kernel(d->dtype == AH_F32 ? k_sample<float, 512> : k_sample<uint16_t, 512>, dim3((unsigned)d->rows), dim3(512), 0, a);
   AH_LAUNCH_CHECK();
   return AH_OK;
 }
