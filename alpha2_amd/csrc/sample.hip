@@ -80,22 +80,24 @@ __device__ __forceinline__ uint64_t wave_running(uint64_t v) {
   v = plus_moved<0x142, 0xa>(v);                 // the last of a row to the next one, of two rows to the next two
   return plus_moved<0x143, 0xc>(v);
 }
-__device__ __forceinline__ uint64_t wave_last(uint64_t v) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+__device__ __forceinline__ uint64_t wave_lane(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
-// the sum over the threads before this one, and over all
+// the sum over the threads before this one, and over all: the waves' sums are added up in the 16 lanes of every row
 template <int THREADS>
 __device__ __forceinline__ uint64_t block_before(uint64_t v, Shared &s, uint64_t &all) {
-  const int wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint64_t upto = wave_running(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) s.part[wave] = upto;
+  if (lane == 63) s.part[wave] = upto;
   __syncthreads();
-  uint64_t before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; w++) { const uint64_t x = s.part[w]; all += x; before += w < wave ? x : 0; }
-  all = same(all);
+  uint64_t waves = (lane & 15) < THREADS / 64 ? s.part[lane & 15] : 0;
+  waves = plus_moved<0x111, 0xf>(waves);
+  waves = plus_moved<0x112, 0xf>(waves);
+  waves = plus_moved<0x114, 0xf>(waves);
+  waves = plus_moved<0x118, 0xf>(waves);
+  all = wave_lane(waves, 63);
+  const uint64_t before = wave ? wave_lane(waves, wave - 1) : 0;
   return before + upto - v;
 }
 template <int THREADS>
@@ -106,15 +108,14 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t v, Shared &s) {
 }
 template <int THREADS>
 __device__ __forceinline__ void block_bounds(float &low, float &high, Shared &s) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   low = -wave_max(-low);
   high = wave_max(high);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) { s.low[threadIdx.x >> 6] = low; s.high[threadIdx.x >> 6] = high; }
+  if (lane == 0) { s.low[wave] = low; s.high[wave] = high; }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; w++) { low = fminf(low, s.low[w]); high = fmaxf(high, s.high[w]); }
-  low = same(low);
-  high = same(high);
+  low = same(-wave_max(-s.low[lane & (THREADS / 64 - 1)]));
+  high = same(wave_max(s.high[lane & (THREADS / 64 - 1)]));
 }
 
 // The n entries of a list in order, into `sorted`.  Up to 256 by counting the larger ones of each, 2 to 16 threads to an entry; more by exchanges,
@@ -153,13 +154,6 @@ __device__ __forceinline__ void sort_list(Shared &s, const uint64_t *list, int n
 }
 
 // ------------------------------------------------------------------------------------------ a row
-struct Past {                                    // a running sum, on from `base`, passes a number or reaches it
-  double target;
-  bool   reach;
-  uint64_t base = 0;
-  __device__ __forceinline__ bool operator()(uint64_t s) const { const double x = (double)(base + s); return reach ? x >= target : x > target; }
-};
-
 template <class T, int THREADS> struct Row {
   static constexpr int N = 16 / sizeof(T);       // logits to a vector
   // The logits before the first whole 16 bytes and behind the last are vectors of one each, so that no other memory is read; all are in the order of the indices.
@@ -199,24 +193,37 @@ template <class T, int THREADS> struct Row {
       for (int j = 0; j < U; j++) if (v0 + j * THREADS < vectors) f(w[j], v0 + j * THREADS);
     }
   }
-  // f(logit, index) for the ones above -infinity for which `hit` holds, which are few: the loop over them is there once
-  template <class Hit, class F>
-  __device__ __forceinline__ void hits(Hit hit, F f) const {
-    constexpr int U = 16 / N;                    // (16 tests written out)
+  // f(logit, index) for the ones in either interval, which are few: a vector is looked into where it has one
+  template <class F>
+  __device__ __forceinline__ void hits(float lo, float hi, float lo2, float hi2, F f) const {
+    constexpr int U = 16 / N;
+    const bool two = lo2 <= hi2;
     for (int v0 = threadIdx.x; v0 < vectors; v0 += THREADS * U) {
       uint4 w[U];
 #pragma unroll
       for (int j = 0; j < U; j++) w[j] = load(v0 + j * THREADS);
-      uint32_t bits = 0;
+      bool some = false;
 #pragma unroll
       for (int j = 0; j < U; j++)
 #pragma unroll
-        for (int i = 0; i < N; i++) { const float l = logit(w[j], i); bits |= l > -INFINITY && hit(l) ? 1u << (j * N + i) : 0u; }
-      while (bits) {
-        const int b = __builtin_ctz(bits);
-        const int n = index(v0 + b / N * THREADS, b % N);
-        f(at(n), n);
-        bits &= bits - 1;
+        for (int i = 0; i < N; i++) { const float l = logit(w[j], i); some |= l == __builtin_amdgcn_fmed3f(l, lo, hi); }
+      if (two)
+#pragma unroll
+        for (int j = 0; j < U; j++)
+#pragma unroll
+          for (int i = 0; i < N; i++) { const float l = logit(w[j], i); some |= l == __builtin_amdgcn_fmed3f(l, lo2, hi2); }
+      if (some) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < U; j++)
+#pragma unroll
+          for (int i = 0; i < N; i++) { const float l = logit(w[j], i); bits |= (l >= lo && l <= hi) || (l >= lo2 && l <= hi2) ? 1u << (j * N + i) : 0u; }
+        while (bits) {
+          const int b = __builtin_ctz(bits);
+          const int n = index(v0 + b / N * THREADS, b % N);
+          f(at(n), n);
+          bits &= bits - 1;
+        }
       }
     }
   }
@@ -227,10 +234,11 @@ struct Weight {
   float top;
   double factor;                                 // 256 log2(e) / temperature
   const double *steps;
-  bool one;
+  uint64_t each;                                 // 0, or what each of them counts
   __device__ __forceinline__ uint64_t operator()(float l) const {
+    if (each) return each;
     const double y = ((double)l - (double)top) * factor;
-    const bool some = y > -44.0 * STEPS;         // (NaN: both are infinite)
+    const bool some = y > -44.0 * STEPS;         // (not NaN)
     constexpr double ROUND = 0x1.8p52;
     const double whole = y + ROUND;
     const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, whole);
@@ -238,10 +246,9 @@ struct Weight {
     const float h = (float)g;
     const double e = fma(g * g, (double)fmaf(h, fmaf(h, 1.0f / 24, 1.0f / 6), 0.5f), g);
     const double step = steps[n & (STEPS - 1)], w = fma(step, e, step);
-    const uint64_t scaled = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(int64_t)((n >> 8) + 43) << 52);
-    const uint64_t units = __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52) - __builtin_bit_cast(uint64_t, 0x1p52);
-    const uint64_t weight = some ? units : l == top ? (uint64_t)UNIT : 0;
-    return one ? 1 : weight;
+    const uint64_t scaled = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(uint32_t)((n >> 8) + 43) << 52);
+    const uint64_t units = __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52) & ((1ull << 52) - 1);
+    return some ? units : 0;
   }
 };
 
@@ -263,11 +270,19 @@ struct Bins {
     const float at = (high - l) * scale;
     return at < (float)(BINS - 1) ? (int)at : BINS - 1;       // (0 x infinity: the last)
   }
-  // the same, asked of one bin
-  __device__ __forceinline__ bool in(float l, int b) const {
-    if (shift >= 0) return (int)((order_of(high) - order_of(l)) >> shift) == b;
-    const float at = (high - l) * scale;
-    return b < BINS - 1 ? at >= (float)b && at < (float)(b + 1) : !(at < (float)(BINS - 1));
+  // logits of bin b lie between these (and, by rounding, others at the ends)
+  __device__ __forceinline__ void around(int b, float low, float &lo, float &hi) const {
+    if (shift >= 0) {
+      hi = of_order(order_of(high) - ((uint32_t)b << shift));
+      const uint64_t end = ((uint64_t)(b + 1) << shift) - 1, span = order_of(high) - order_of(low);
+      lo = of_order(order_of(high) - (uint32_t)(end < span ? end : span));
+      return;
+    }
+    const float wide = 1.0f / scale, slack = 4e-7f * (fabsf(high) + (b + 1) * wide);      // several roundings of each of the two
+    lo = high - (b + 1) * wide - slack;
+    hi = fminf(high, high - b * wide + slack);
+    if (b == BINS - 1 || !(lo >= low)) lo = low;
+    if (!(hi >= low)) hi = high;                 // (no width: every bin is the first or the last)
   }
 };
 static_assert(BINS == 1 << 11, "the shift of a bin's bins");
@@ -285,15 +300,15 @@ __device__ __forceinline__ uint64_t sum_bins(Shared &s, int level) {
   __syncthreads();
   return all;
 }
-// Where in s.bins[level] running sums, on from `base`, pass: the bin into s.found, the sum before it into s.found_before.
+// Where in s.bins[level] running sums, on from `base`, reach `mark`: the bin into s.found, the sum before it into s.found_before.
 template <int THREADS>
-__device__ __forceinline__ void find_bin(Shared &s, int level, uint64_t base, const Past &past) {
+__device__ __forceinline__ void find_bin(Shared &s, int level, uint64_t base, uint64_t mark) {
   constexpr int EACH = BINS / THREADS;
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
     const int b = EACH * threadIdx.x + i;
     const uint64_t before = base + (b ? s.bins[level][b - 1] : 0), upto = base + s.bins[level][b];
-    if (!past(before) && past(upto)) { s.found = b; s.found_before = before; }
+    if (before < mark && upto >= mark) { s.found = b; s.found_before = before; }
   }
   __syncthreads();
 }
@@ -306,7 +321,7 @@ struct Found {
 
 template <class T, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
-  constexpr int WAVES = THREADS / 64, EACH = LIST / THREADS, N = Row<T, THREADS>::N;
+  constexpr int WAVES = THREADS / 64, EACH = LIST / THREADS, N = Row<T, THREADS>::N, UNDER_WAY = 2;
   __shared__ Shared s;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const int64_t r = blockIdx.x;
@@ -344,16 +359,21 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
   block_bounds<THREADS>(low, top, s);
   if (top == -INFINITY) { if (t == 0) answer(0, NAN); return; }
 
-  Weight weight{top, STEPS * 1.44269504088896340736 / (double)temperature, s.steps, false};
-  const bool nucleus = p > 0.f && p < 1.f, cut = k > 0 && k < row.V;
+  // An infinite largest: there is nothing but those, and each weighs 1.
+  const bool infinite = top == INFINITY;
+  float bound = infinite ? top : low;            // what top_k leaves is not below it
+  Weight weight{top, STEPS * 1.44269504088896340736 / (double)temperature, s.steps, infinite ? (uint64_t)UNIT : 0};
+  const uint64_t unit = weight.each;
+  const bool nucleus = p > 0.f && p < 1.f, cut = k > 0 && k < row.V, some_drop = least_p > 0.f && temperature < INFINITY;
   // a weight of at least min_p
-  const double drop = least_p > 0.f && temperature < INFINITY ? (double)temperature * log((double)fminf(least_p, 1.f)) : -INFINITY;
-  auto enough = [&](float l) { return l == top || (double)l - (double)top >= drop; };
-  const double draw = fmin(fmax((double)u, 0.0), 1.0);
+  const double drop = some_drop ? (double)temperature * log((double)fminf(least_p, 1.f)) : -INFINITY;
+  auto enough = [&](float l) { return !some_drop || l == top || (double)l - (double)top >= drop; };
+  // The sums that running sums have to reach: the nucleus's, and the token's, which passes the given number; where rounding, or a number of 1, leaves nothing
+  // beyond it, that is the last that weighs something.
+  auto nucleus_mark = [&](uint64_t all) { const uint64_t m = (uint64_t)ceil((double)p * (double)all); return m < 1 ? 1 : m > all ? all : m; };
+  auto token_mark = [&](uint64_t all) { const uint64_t m = (uint64_t)(fmin(fmax((double)u, 0.0), 1.0) * (double)all); return m < all ? m + 1 : all; };
   // what one thread finds: the token and the sum of what is kept
   auto finish = [&](uint64_t entry, uint64_t all) { s.answer = entry; s.kept = all; };
-  // the number that the walk has to pass: where rounding, or a number of 1, leaves nothing beyond it, the last that weighs something
-  auto walk = [&](uint64_t all) { const double target = draw * (double)all; return (double)all > target ? Past{target, false} : Past{(double)all, true}; };
   auto list = [&](int which, float l, int index) {
     const int at = atomicAdd(&s.listed[which], 1);
     if (at < LIST) s.list[which][at] = entry_of(l, index);
@@ -362,7 +382,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
   auto choose = [&] {
     const bool small = row.V <= SMALL;
     if (small || (cut && k <= FEW)) {
-      if (small) row.hits([](float) { return true; }, [&](float l, int index) { list(0, l, index); });
+      if (small) row.hits(bound, top, INFINITY, -INFINITY, [&](float l, int index) { list(0, l, index); });
       else {
         // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
         float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
@@ -372,35 +392,36 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
         __syncthreads();
         if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
         __syncthreads();
-        const bool every = sum_bins<THREADS>(s, 0) < (uint64_t)k;    // fewer maxima than that: all of the row are candidates
-        find_bin<THREADS>(s, 0, 0, Past{(double)k, true});
-        const float to = every ? INFINITY : (float)(same(s.found) + 1);        // (the last bin has no end)
-        row.hits([&](float l) { return (bin.high - l) * bin.scale < to || to >= (float)BINS; }, [&](float l, int index) { list(0, l, index); });
+        const bool every = sum_bins<THREADS>(s, 0) < (uint64_t)k;  // fewer maxima than that: all of the row are candidates
+        find_bin<THREADS>(s, 0, 0, (uint64_t)k);
+        const int last = every ? BINS - 1 : same(s.found);
+        float lo = bound, hi;
+        if (last < BINS - 1) bin.around(last, bound, lo, hi);      // (the last bin has no end)
+        row.hits(lo, top, INFINITY, -INFINITY, [&](float l, int index) { if (bin(l) <= last) list(0, l, index); });
       }
       __syncthreads();
       const int n = same(s.listed[0]);
       if (n <= LIST) {
         sort_list<THREADS>(s, s.list[0], n);
-        const uint32_t kth = cut && n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u;
-        if (n <= 64) {                             // a wave alone
+        const uint32_t kth = cut && n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u, lowest = max(kth, order_of(bound));
+        if (n <= 64) {                           // a wave alone
           if (wave) return;
           const uint64_t e = lane < n ? s.sorted[lane] : 0;
           const float l = entry_logit(e);
           const uint64_t x = weight(l);
-          uint64_t w = lane < n && (uint32_t)(e >> 32) >= kth ? x : 0, upto = wave_running(w), all = wave_last(upto);
-          const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
-          w = !end(upto - w) && enough(l) ? w : 0;
+          uint64_t w = lane < n && (uint32_t)(e >> 32) >= lowest ? x : 0, upto = wave_running(w), all = wave_lane(upto, 63);
+          w = (!nucleus || upto - w < nucleus_mark(all)) && enough(l) ? w : 0;
           upto = wave_running(w);
-          all = wave_last(upto);
-          if (!nucleus) {                          // by index
+          all = wave_lane(upto, 63);
+          if (!nucleus) {                        // by index
             s.bins[0][lane] = (uint32_t)e;
             s.bins[1][lane] = w;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             upto = 0;
             for (int j = 0; j < n; j++) { const uint64_t other = s.bins[0][j], more = s.bins[1][j]; upto += other >= (uint32_t)e ? more : 0; }
           }
-          const Past past = walk(all);
-          if (!past(upto - w) && past(upto)) finish(e, all);
+          const uint64_t mark = token_mark(all);
+          if (upto - w < mark && upto >= mark && w) finish(e, all);
           return;
         }
         uint64_t e[EACH], w[EACH], sum = 0, all;
@@ -409,26 +430,25 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
           const int at = EACH * t + i;
           e[i] = at < n ? s.sorted[at] : 0;
           const uint64_t x = weight(entry_logit(e[i]));
-          w[i] = at < n && (uint32_t)(e[i] >> 32) >= kth ? x : 0;
+          w[i] = at < n && (uint32_t)(e[i] >> 32) >= lowest ? x : 0;
           sum += w[i];
         }
-        uint64_t before = block_before<THREADS>(sum, s, all);
-        const Past end{nucleus ? (double)p * (double)all : INFINITY, true};
-        uint64_t number = 0;
+        uint64_t before = block_before<THREADS>(sum, s, all), number = 0;
+        const uint64_t end = nucleus ? nucleus_mark(all) : ~0ull;
         sum = 0;
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          const bool stays = !end(before) && enough(entry_logit(e[i]));
+          const bool stays = before < end && enough(entry_logit(e[i]));
           before += w[i];
           w[i] = stays ? w[i] : 0;
           number += w[i] != 0;
         }
-        if (!nucleus) {                            // by index: the list again with the index first and the place in the order behind it
+        if (!nucleus) {                          // by index: the list again with the index first and the place in the order behind it
           uint64_t at = block_before<THREADS>(number, s, number);
 #pragma unroll
           for (int i = 0; i < EACH; i++) {
             if (w[i]) s.list[0][at++] = (uint64_t)(uint32_t)e[i] << 32 | (uint32_t)(EACH * t + i);
-            s.bins[0][EACH * t + i] = e[i];        // (what was sorted by logit is needed once more)
+            s.bins[0][EACH * t + i] = e[i];      // (what was sorted by logit is needed once more)
             s.bins[1][EACH * t + i] = w[i];
           }
           sort_list<THREADS>(s, s.list[0], (int)number);
@@ -443,10 +463,10 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
 #pragma unroll
         for (int i = 0; i < EACH; i++) sum += w[i];
         before = block_before<THREADS>(sum, s, all);
-        const Past past = walk(all);
+        const uint64_t mark = token_mark(all);
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-          if (!past(before) && past(before + w[i])) finish(e[i], all);
+          if (before < mark && before + w[i] >= mark) finish(e[i], all);
           before += w[i];
         }
         return;
@@ -454,15 +474,13 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
     }
 
     // Descents, from the largest down: to the k-th largest, to where the nucleus ends, to the token.
-    float bound = low;                             // what top_k leaves is not below it
-    uint64_t all = 0;
-    Past past{0.0, true};
-    Found f{top, 0, 0, 0};
+    uint64_t all = 0, mark = (uint64_t)k;
+    Found f{bound, 0, 0, 0};
     enum { KTH, END, TOKEN, NONE };
     int goal = cut ? KTH : nucleus ? END : NONE;
-    Bins bin(low, top, INFINITY);
+    Bins bin(bound, top, INFINITY);
     // The row's own bins whose members are in the two lists: the one the nucleus ends in and, so that the row need not be gone over again, the one the
-    // token is in if it ends with that bin.
+    // token is in if the nucleus ends with that bin.
     int have[2] = {-1, -1}, members[2] = {0, 0};
     for (int turn = 0; turn < 3 && goal != NONE; turn++) {
       float least = bound, most = top;
@@ -471,56 +489,65 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
       uint64_t base = 0, of_enough = 0;
       for (int level = 0; level < 5; level++) {
         const int l1 = level ? 1 : 0;
-        if (level || goal != TOKEN) {              // (the token's are those of the nucleus)
-          weight.one = goal == KTH;
+        if (level || goal != TOKEN) {            // (the token's are those of the nucleus)
+          weight.each = goal == KTH ? 1 : unit;
           bin = level ? Bins(least, most) : Bins(bound, top, goal == KTH ? INFINITY : 31.f * temperature);
           __syncthreads();
           for (int i = t; i < BINS; i += THREADS) s.bins[l1][i] = 0;
           __syncthreads();
           uint64_t sum = 0;
-          row.template each<8 / N>([&](const uint4 &w, int) {
+          row.template each<UNDER_WAY>([&](const uint4 &w, int) {
+            uint64_t x[N];                       // (all of a vector's at once, so that they are under way side by side)
 #pragma unroll
             for (int i = 0; i < N; i++) {
               const float l = logit(w, i);
-              if (l >= least && l <= most) {       // (not NaN, and above -infinity like those)
-                const uint64_t x = weight(l);
-                sum += enough(l) ? x : 0;
-                if (x) atomicAdd((unsigned long long *)&s.bins[l1][bin(l)], (unsigned long long)x);
-              }
+              const uint64_t y = weight(l);
+              x[i] = l >= least && l <= most ? y : 0;                // (not NaN, and above -infinity like those)
             }
+            if (some_drop)
+#pragma unroll
+              for (int i = 0; i < N; i++) sum += enough(logit(w, i)) ? x[i] : 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) if (x[i]) atomicAdd((unsigned long long *)&s.bins[l1][bin(logit(w, i))], (unsigned long long)x[i]);
           });
           __syncthreads();
           const uint64_t total = sum_bins<THREADS>(s, l1);
           if (!level) {
-            if (goal == KTH && total <= (uint64_t)k) break;            // nothing to cut
-            past = Past{goal == KTH ? (double)k : (double)p * (double)total, true};
-            if (goal == END) of_enough = block_sum<THREADS>(sum, s);
+            if (goal == KTH && total <= (uint64_t)k) break;          // nothing to cut: f is the lowest
+            if (goal == END) mark = nucleus_mark(total);
+            of_enough = some_drop && goal == END ? block_sum<THREADS>(sum, s) : total;
           }
         }
         __syncthreads();
         if (t == 0 && (level || goal != TOKEN)) s.listed[0] = s.listed[1] = 0;
-        find_bin<THREADS>(s, l1, base, past);
+        find_bin<THREADS>(s, l1, base, mark);
         const int b = same(s.found);
         base = same(s.found_before);
         int which = 0, n = 0;
         const bool listed = !level && goal == TOKEN && (b == have[0] || b == have[1]);
+        float lo, hi;
+        bin.around(b, least, lo, hi);
         if (listed) {
           which = b == have[0] ? 0 : 1;
           n = members[which];
         } else {
           int too = -1;
+          float lo2 = INFINITY, hi2 = -INFINITY;
           if (!level && goal == END) {
-            const Past then = walk(same(s.bins[0][b]));
+            const uint64_t then = token_mark(same(s.bins[0][b]));
             __syncthreads();
             find_bin<THREADS>(s, 0, 0, then);
             too = same(s.found);
-          } else if (!level && goal == TOKEN) {    // (neither list: the first is made anew)
+            if (too != b) bin.around(too, least, lo2, hi2);
+          } else if (!level && goal == TOKEN) {  // (neither list: the first is made anew)
             __syncthreads();
             if (t == 0) s.listed[0] = 0;
             __syncthreads();
           }
-          row.hits([&](float l) { return l >= least && l <= most && (bin.in(l, b) || (too >= 0 && bin.in(l, too))); },
-                   [&](float l, int index) { list(bin.in(l, b) ? 0 : 1, l, index); });
+          row.hits(lo, hi, lo2, hi2, [&](float l, int index) {
+            const int at = bin(l);
+            if (at == b || at == too) list(at == b ? 0 : 1, l, index);
+          });
           __syncthreads();
           n = same(s.listed[0]);
           if (!level && goal == END) {
@@ -531,7 +558,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
           } else if (goal == END) have[0] = -1;
         }
         if (n <= LIST) {
-          if (!(listed && which == 0)) sort_list<THREADS>(s, s.list[which], n);        // (the nucleus's is sorted)
+          if (!(listed && which == 0)) sort_list<THREADS>(s, s.list[which], n);      // (the nucleus's is sorted)
           uint64_t w[EACH], sum = 0, dummy;
 #pragma unroll
           for (int i = 0; i < EACH; i++) {
@@ -543,10 +570,11 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
           uint64_t before = base + block_before<THREADS>(sum, s, dummy);
 #pragma unroll
           for (int i = 0; i < EACH; i++) {
-            if (!past(before) && past(before + w[i])) {
+            if (before < mark && before + w[i] >= mark) {
               const uint64_t e = s.sorted[EACH * t + i];
               if (goal == TOKEN) finish(e, all);
-              else { s.found_entry = e; s.found_before = before + w[i]; }
+              s.found_entry = e;
+              s.found_before = before + w[i];
             }
             before += w[i];
           }
@@ -556,15 +584,21 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
           f = Found{entry_logit(e), entry_index(e), same(s.found_before), 0};
           break;
         }
-        float lo = INFINITY, hi = -INFINITY;
-        row.hits([&](float l) { return l >= least && l <= most && bin.in(l, b); }, [&](float l, int) { lo = fminf(lo, l); hi = fmaxf(hi, l); });
+        const float from = lo, to = hi;
+        lo = INFINITY;
+        hi = -INFINITY;
+        row.hits(from, to, INFINITY, -INFINITY, [&](float l, int) {
+          const bool in = bin(l) == b;
+          lo = in ? fminf(lo, l) : lo;
+          hi = in ? fmaxf(hi, l) : hi;
+        });
         block_bounds<THREADS>(lo, hi, s);
-        if (lo == hi) {                            // equal ones: how many of them it takes
+        if (lo == hi) {                          // equal ones: how many of them it takes
           const uint64_t w = same(weight(lo));
           uint32_t few = 1, many = (uint32_t)n;
           for (int i = 0; i < 20 && few < many; i++) {
             const uint32_t middle = few + (many - few) / 2;
-            if (past(base + middle * w)) many = middle; else few = middle + 1;
+            if (base + middle * w >= mark) many = middle; else few = middle + 1;
           }
           f = Found{lo, -1, base + few * w, base};
           break;
@@ -573,21 +607,19 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
         most = hi;
       }
       if (goal == KTH) {
-        bound = past.target > 0.0 ? f.logit : low;
-        past = Past{0.0, true};
+        bound = f.logit;
         goal = nucleus ? END : NONE;
       } else if (goal == END) {
         all = enough(f.logit) ? f.upto : of_enough;
-        past = walk(all);
+        mark = token_mark(all);
         bin = Bins(bound, top, 31.f * temperature);
         goal = TOKEN;
       } else goal = NONE;
     }
-    weight.one = false;
+    weight.each = unit;
 
     // By index: all that is kept where there is no nucleus, or the equal ones among which the token is.
-    const bool equal = nucleus;
-    const float from = equal ? f.logit : bound, to = equal ? f.logit : top;
+    const float from = nucleus ? f.logit : bound, to = nucleus ? f.logit : top;
     const int runs = (row.vectors + 63) / 64;
     __syncthreads();
     for (int n0 = wave; n0 < runs; n0 += 2 * WAVES) {
@@ -597,10 +629,16 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         uint64_t sum = 0;
+        bool some = false;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-          const float l = logit(w[j], i);
-          if (l >= from && l <= to && enough(l)) sum += weight(l);
+        for (int i = 0; i < N; i++) { const float l = logit(w[j], i); some |= l >= from && l <= to && enough(l); }
+        if (__any(some)) {
+#pragma unroll
+          for (int i = 0; i < N; i++) {
+            const float l = logit(w[j], i);
+            const uint64_t x = weight(l);
+            sum += l >= from && l <= to && enough(l) ? x : 0;
+          }
         }
         sum = wave_running(sum);
         if (lane == 63 && n0 + j * WAVES < runs) s.runs[n0 + j * WAVES] = sum;
@@ -611,19 +649,18 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
     uint64_t sum = 0, total;
     for (int i = 0; i < each; i++) sum += r0 + i < runs ? s.runs[r0 + i] : 0;
     uint64_t before = block_before<THREADS>(sum, s, total);
-    if (equal) past.base = f.before;
-    else {
+    if (!nucleus) {
       all = total;
-      past = walk(all);
-    }
+      mark = token_mark(all);
+    } else mark -= f.before;
     for (int i = 0; i < each; i++) {
       const uint64_t x = r0 + i < runs ? s.runs[r0 + i] : 0;
-      if (!past(before) && past(before + x)) { s.found = r0 + i; s.found_before = before; }
+      if (before < mark && before + x >= mark) { s.found = r0 + i; s.found_before = before; }
       before += x;
     }
     __syncthreads();
     if (wave) return;
-    const int v = same(s.found) * 64 + lane;       // the run again
+    const int v = same(s.found) * 64 + lane;     // the run again
     const uint4 w = row.load(v);
     uint64_t x[N], mass = 0;
 #pragma unroll
@@ -638,7 +675,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
     float l = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const bool here = !past(upto) && past(upto + x[i]);
+      const bool here = upto < mark && upto + x[i] >= mark;
       upto += x[i];
       token = here ? row.index(v, i) : token;
       l = here ? logit(w, i) : l;
