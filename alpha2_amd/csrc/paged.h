@@ -11,8 +11,8 @@
 
 namespace ah {
 
-// Whole quotients by a number that is the same for a launch, of numerators below 2^31: with 2^(shift - 1) < divisor <= 2^shift and
-// magic = ceil(2^(31 + shift) / divisor) < 2^32 the product n * magic is n * 2^(31 + shift) / divisor and less than 2^(31 + shift) / divisor more.
+// Whole quotients by a number below 2^31 that is the same for a launch, of numerators below 2^31: with 2^(shift - 1) < divisor <= 2^shift and
+// magic = ceil(2^(31 + shift) / divisor) < 2^32 (`shift` here has the 31 in it) the product n * magic is n * 2^(31 + shift) / divisor and less than 2^(31 + shift) / divisor more.
 struct Quotient {
   uint32_t divisor, magic;
   int32_t  shift;

@@ -32,22 +32,12 @@ int32_t paged_cache(const char *who, const AhPages *p, int32_t rows, PagedCache 
 
 namespace {
 
-// The sequence that new row `row` belongs to, by a whole wave: the last one that starts at or before it; -1: none.  `position`: its
-// position in it, negative where the sequence has fewer positions than new tokens.
-__device__ __forceinline__ int sequence_at(const PagedCache &c, int row, int &position) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int s0 = 0; s0 < c.seqs; s0 += 64) {
-    const int s = s0 + lane;
-    before += __popcll(__ballot(s < c.seqs && c.starts[s < c.seqs ? s : 0] <= row));
-  }
-  if (before == 0) return -1;
-  const Sequence s = sequence_of(c.starts[before - 1], c.starts[before], c.lens[before - 1], c.rows);
-  position = s.len - s.count + (row - s.first);
-  return row >= s.first && row < s.first + s.count ? before - 1 : -1;
-}
-
 // ------------------------------------------------------------------------------------------ append
+// A workgroup takes a few rows.  Its first wave finds out where they go, all at once: three loads one after the other (the starts, the length and the starts
+// of each row's sequence, the table's entry), whatever the rows.  Then every thread takes 16-byte pieces of heads, a pair of them where the turned features
+// of a pair lie half a rotation apart.
+constexpr int MOST_ROWS = 16;
+
 struct AppendArgs {
   PagedCache c;
   void *k_pages, *v_pages;
@@ -55,35 +45,153 @@ struct AppendArgs {
   void *rotated;
   const float *rotary;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, r_st, r_sh;
-  int32_t heads, kv_heads, head_dim, rot, rot_rows, neighbours;
+  int32_t heads, kv_heads, head_dim, rot, rot_rows;
+  int32_t group;              // rows of a workgroup
+  Quotient of_row;            // items of a row: those of the turned heads, q before k, then those of v
+  Quotient of_turned;         // items of a turned head
+  Quotient of_head;           // 16-byte pieces of a head
 };
+// How the turned heads are cut into items.  NONE: no rotation; HALVES: a piece of each half of the rotation, and the pieces behind it; NEIGHBOURS: pieces; ODD:
+// two features, where the halves are no whole pieces.
+enum { NONE, HALVES, NEIGHBOURS, ODD };
 
-// A wave to a row, a feature to a lane.
-template <class T>
-__global__ __launch_bounds__(64) void k_paged_append(AppendArgs a) {
-  const int row = blockIdx.x, lane = threadIdx.x;
-  int position;
-  const int seq = sequence_at(a.c, row, position);
-  if (seq < 0) return;
-  const int64_t place = position_place(a.c, seq, position);
-  const int half = a.rot / 2;
-  for (int h = 0; h < a.heads + 2 * a.kv_heads; h++) {
-    const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + a.kv_heads;
-    if (is_q ? a.rot == 0 : place < 0) continue;
-    const int kh = is_k ? h - a.heads : h - a.heads - a.kv_heads;
-    const T *src = is_q ? (const T *)a.q + row * a.q_st + h * a.q_sh : is_k ? (const T *)a.k + row * a.k_st + kh * a.k_sh : (const T *)a.v + row * a.v_st + kh * a.v_sh;
-    T *dst = is_q ? (T *)a.rotated + row * a.r_st + h * a.r_sh : (T *)(is_k ? a.k_pages : a.v_pages) + place + kh * a.c.head_stride;
-    const int rot = is_q || is_k ? a.rot : 0;
-    for (int i = lane; i < rot / 2; i += 64) {
-      const int f0 = a.neighbours ? 2 * i : i, f1 = a.neighbours ? 2 * i + 1 : i + half;
-      float cosine = NAN, sine = NAN;
-      if (position >= 0 && position < a.rot_rows) { cosine = a.rotary[(int64_t)position * a.rot + i]; sine = a.rotary[(int64_t)position * a.rot + half + i]; }
-      const float x = Io<T>::ld(src, f0), y = Io<T>::ld(src, f1);
-      Io<T>::st(dst, f0, x * cosine - y * sine);
-      Io<T>::st(dst, f1, y * cosine + x * sine);
-    }
-    for (int f = rot + lane; f < a.head_dim; f += 64) dst[f] = src[f];
+template <class T> struct Piece;
+template <> struct Piece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const float *p, float (&x)[4]) { const float4 w = *reinterpret_cast<const float4 *>(p); x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w; }
+  static __device__ __forceinline__ void put(float *p, const float (&x)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+};
+template <> struct Piece<uint16_t> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint16_t *p, float (&x)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
   }
+  static __device__ __forceinline__ void put(uint16_t *p, const float (&x)[8]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+  }
+};
+__device__ __forceinline__ void turn(float &a, float &b, float cosine, float sine) {
+  const float x = a;
+  a = fmaf(x, cosine, -(b * sine));
+  b = fmaf(b, cosine, x * sine);
+}
+
+template <class T, int MODE>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
+  constexpr int N = Piece<T>::N;
+  __shared__ int64_t places[MOST_ROWS];         // elements from the start of the pages, negative: nowhere
+  __shared__ int32_t positions[MOST_ROWS];      // INT32_MIN: a row of no sequence
+  const int first = blockIdx.x * a.group, rows = min(a.group, a.c.rows - first);
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    int before = 0;                             // lane r: starts at or before row first + r
+    for (int s0 = 0; s0 < a.c.seqs; s0 += 64) {
+      const int start = s0 + lane < a.c.seqs ? a.c.starts[s0 + lane] : INT32_MAX;
+      for (int r = 0; r < rows; r++) {
+        const int n = __popcll(__ballot(start <= first + r));
+        before += lane == r ? n : 0;
+      }
+    }
+    if (lane < rows) {
+      int64_t place = -1;
+      int32_t position = INT32_MIN;
+      if (before > 0) {
+        const int seq = before - 1, row = first + lane;
+        const Sequence s = sequence_of(a.c.starts[seq], a.c.starts[seq + 1], a.c.lens[seq], a.c.rows);
+        if (row >= s.first && row < s.first + s.count) {
+          position = s.len - s.count + (row - s.first);
+          place = position_place(a.c, seq, position);
+        }
+      }
+      places[lane] = place;
+      positions[lane] = position;
+    }
+  }
+  __syncthreads();
+  const int half = a.rot / 2;
+  const uint32_t turned = MODE == NONE ? 0u : (uint32_t)(a.heads + a.kv_heads) * a.of_turned.divisor;
+  for (uint32_t i = threadIdx.x; i < (uint32_t)rows * a.of_row.divisor; i += 256) {
+    const uint32_t r = quotient(i, a.of_row), item = i - r * a.of_row.divisor;
+    const int64_t place = places[r], row = first + r;
+    const int32_t position = positions[r];
+    if (position == INT32_MIN) continue;
+    if (MODE != NONE && item < turned) {
+      const uint32_t h = quotient(item, a.of_turned), part = item - h * a.of_turned.divisor;
+      const bool is_q = (int)h < a.heads;
+      if (!is_q && place < 0) continue;
+      const int kh = (int)h - a.heads;
+      const T *src = is_q ? (const T *)a.q + row * a.q_st + h * a.q_sh : (const T *)a.k + row * a.k_st + kh * a.k_sh;
+      T *dst = is_q ? (T *)a.rotated + row * a.r_st + h * a.r_sh : (T *)a.k_pages + place + kh * a.c.head_stride;
+      const bool known = position >= 0 && position < a.rot_rows;
+      const float *table = a.rotary + (known ? (int64_t)position * a.rot : 0);
+      if constexpr (MODE == HALVES) {
+        const int f = (int)part * N;
+        if (f < half) {
+          float x[N], y[N];
+          Piece<T>::get(src + f, x);
+          Piece<T>::get(src + f + half, y);
+#pragma unroll
+          for (int e = 0; e < N; e += 4) {
+            float4 c = make_float4(NAN, NAN, NAN, NAN), s = c;
+            if (known) { c = *reinterpret_cast<const float4 *>(table + f + e); s = *reinterpret_cast<const float4 *>(table + half + f + e); }
+            turn(x[e], y[e], c.x, s.x); turn(x[e + 1], y[e + 1], c.y, s.y); turn(x[e + 2], y[e + 2], c.z, s.z); turn(x[e + 3], y[e + 3], c.w, s.w);
+          }
+          Piece<T>::put(dst + f, x);
+          Piece<T>::put(dst + f + half, y);
+        } else *reinterpret_cast<uint4 *>(dst + f + half) = *reinterpret_cast<const uint4 *>(src + f + half);
+      } else if constexpr (MODE == NEIGHBOURS) {
+        const int f = (int)part * N;
+        if (f < a.rot) {
+          float x[N];
+          Piece<T>::get(src + f, x);
+#pragma unroll
+          for (int e = 0; e < N; e += 2)
+            if (f + e < a.rot) turn(x[e], x[e + 1], known ? table[(f + e) / 2] : NAN, known ? table[half + (f + e) / 2] : NAN);
+          Piece<T>::put(dst + f, x);
+        } else *reinterpret_cast<uint4 *>(dst + f) = *reinterpret_cast<const uint4 *>(src + f);
+      } else {
+        const int p = (int)part, f = p < half ? p : 2 * p, g = p < half ? p + half : 2 * p + 1;
+        if (p < half) {
+          float x = Io<T>::ld(src, f), y = Io<T>::ld(src, g);
+          turn(x, y, known ? table[p] : NAN, known ? table[half + p] : NAN);
+          Io<T>::st(dst, f, x);
+          Io<T>::st(dst, g, y);
+        } else { dst[f] = src[f]; dst[g] = src[g]; }
+      }
+    } else if (place >= 0) {
+      const uint32_t rest = item - turned, h = quotient(rest, a.of_head), f = (rest - h * a.of_head.divisor) * N;
+      const bool is_k = MODE == NONE && (int)h < a.kv_heads;
+      const int kh = MODE == NONE && !is_k ? (int)h - a.kv_heads : (int)h;
+      const T *src = is_k ? (const T *)a.k + row * a.k_st + kh * a.k_sh : (const T *)a.v + row * a.v_st + kh * a.v_sh;
+      T *dst = (T *)(is_k ? a.k_pages : a.v_pages) + place + kh * a.c.head_stride;
+      *reinterpret_cast<uint4 *>(dst + f) = *reinterpret_cast<const uint4 *>(src + f);
+    }
+  }
+}
+template <class T>
+int32_t append(AppendArgs &a, bool neighbours) {
+  constexpr int N = Piece<T>::N;
+  const uint32_t pieces = (uint32_t)(a.head_dim / N), half = (uint32_t)(a.rot / 2);
+  const int mode = a.rot == 0 ? NONE : neighbours ? NEIGHBOURS : half % N == 0 ? HALVES : ODD;
+  a.of_head = quotient_by(pieces);
+  a.of_turned = quotient_by(mode == HALVES ? pieces - half / N : mode == ODD ? (uint32_t)a.head_dim / 2 : pieces);
+  const int64_t items = mode == NONE ? (int64_t)2 * a.kv_heads * pieces
+                                     : (int64_t)(a.heads + a.kv_heads) * a.of_turned.divisor + (int64_t)a.kv_heads * pieces;
+  if (items > INT32_MAX / MOST_ROWS) return fail(AH_ERR_UNSUPPORTED, "ah_paged_append: %lld pieces to a row", (long long)items);
+  a.of_row = quotient_by((uint32_t)items);
+  const int64_t want = cdiv(2048, items), fill = cdiv(a.c.rows, (int64_t)4 * num_cus());
+  a.group = (int32_t)(want < fill ? want : fill);
+  if (a.group > MOST_ROWS) a.group = MOST_ROWS;
+  const dim3 grid((unsigned)cdiv(a.c.rows, a.group));
+  if (mode == NONE) launch_kernel(k_paged_append<T, NONE>, grid, dim3(256), 0, a);
+  else if (mode == HALVES) launch_kernel(k_paged_append<T, HALVES>, grid, dim3(256), 0, a);
+  else if (mode == NEIGHBOURS) launch_kernel(k_paged_append<T, NEIGHBOURS>, grid, dim3(256), 0, a);
+  else launch_kernel(k_paged_append<T, ODD>, grid, dim3(256), 0, a);
+  AH_LAUNCH_CHECK();
+  return AH_OK;
 }
 
 }  // namespace
@@ -115,10 +223,8 @@ int32_t ah_paged_append(const AhPages *p, const AhPagedAppend *d) {
   a.rotated = dp<void>(d->rotated); a.rotary = dp<float>(d->rotary);
   a.q_st = d->q_st; a.q_sh = d->q_sh; a.k_st = d->k_st; a.k_sh = d->k_sh; a.v_st = d->v_st; a.v_sh = d->v_sh; a.r_st = d->r_st; a.r_sh = d->r_sh;
   a.heads = d->rot_dim > 0 ? d->heads : 0; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
-  a.rot = d->rot_dim; a.rot_rows = d->rot_rows; a.neighbours = d->rot_neighbours != 0;
-  launch_kernel(p->dtype == AH_F32 ? k_paged_append<float> : k_paged_append<uint16_t>, dim3((unsigned)d->rows), dim3(64), 0, a);
-  AH_LAUNCH_CHECK();
-  return AH_OK;
+  a.rot = d->rot_dim; a.rot_rows = d->rot_rows;
+  return p->dtype == AH_F32 ? append<float>(a, d->rot_neighbours != 0) : append<uint16_t>(a, d->rot_neighbours != 0);
 }
 
 }  // extern "C"

@@ -30,6 +30,10 @@ int main() {
       }
     CHECK(quotient(0x7fffffffu, q) == 0x7fffffffu / d);
   }
+  for (uint32_t d : {65537u, 98304u, 131071u, 1000003u, 1u << 26, 134217727u, 0x7fffffffu}) {
+    const Quotient q = quotient_by(d);
+    for (uint32_t n : {0u, d - 1, d, d + 1 < 0x7fffffffu ? d + 1 : d, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1, 0x7fffffffu}) CHECK(quotient(n, q) == n / d);
+  }
   // places: pages of 5 rows, two sequences of 3 entries; a page outside the array and a position past the table have none
   const int32_t table[6] = {2, 0, 7, -1, 1, 2147483647};
   PagedCache c{};
