@@ -17,8 +17,7 @@
 //
 // Masked places.  A position past a column's limit has its score replaced by -infinity, whatever it was.  Its value would still meet a weight of 0
 // in the matrix product, and 0 x infinity is NaN; so rows past the part's end are zeros, and where some columns see a row that others do
-// not (tiles on the diagonal) values that are not finite are taken out of the product and put back by two products of 0s and 1s that count,
-// for each column, the +infinities (and NaN) and -infinities (and NaN) it does see.
+// not (tiles on the diagonal) values that are not finite are taken as 0 in the product and added, as they are, to the columns that see them, behind the loop.
 // A page that the table has wrong reads as NaN keys and zero values: whoever sees it gets NaN, nobody else.
 #include "attention_bf16_tiles.h"
 #include "paged.h"
@@ -139,27 +138,28 @@ __device__ __forceinline__ bool has_special(bf16x8 v) {
   for (int i = 0; i < 4; i++) any |= (w[i] & 0x7f807f80u) + 0x00800080u;
   return (any & 0x80008000u) != 0;
 }
-// v without them, and 1 where it is +infinity (-infinity) or NaN
-__device__ __forceinline__ void take_special(bf16x8 v, bf16x8 &rest, bf16x8 &up, bf16x8 &down) {
-  typedef __attribute__((ext_vector_type(8))) uint16_t u16x8;
-  const u16x8 w = __builtin_bit_cast(u16x8, v);
-  u16x8 r, p, n;
+__device__ __forceinline__ bf16x8 finite_of(bf16x8 v) {             // 0 in their place
+  u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const bool special = (w[i] & 0x7f80) == 0x7f80;
-    r[i] = special ? 0 : w[i];
-    p[i] = special && w[i] != 0xff80 ? 0x3f80 : 0;
-    n[i] = special && w[i] != 0x7f80 ? 0x3f80 : 0;
+  for (int i = 0; i < 4; i++) {
+    const uint32_t low = (w[i] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu, high = (w[i] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
+    w[i] &= low | high;
   }
-  rest = __builtin_bit_cast(bf16x8, r); up = __builtin_bit_cast(bf16x8, p); down = __builtin_bit_cast(bf16x8, n);
+  return __builtin_bit_cast(bf16x8, w);
 }
-__device__ __forceinline__ bf16x8 ones_where_seen(bf16x8 p) {
-  bf16x8 r;
-#pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = (float)p[i] == 0.f ? (__bf16)0.f : (__bf16)1.f;
-  return r;
+__device__ __forceinline__ float special_of(float v, bool seen) { return seen && !(fabsf(v) < INFINITY) ? v : 0.f; }
+// The same address, as far as the compiler knows another one: what the seldom taken path reads from LDS is not kept in registers for the usual one.
+__device__ __forceinline__ const char *apart(const char *p) {
+  int offset = 0;
+  asm volatile("" : "+v"(offset));
+  return p + offset;
 }
-__device__ __forceinline__ float put_back(float o, float up, float down) { return o + (up > 0.f ? INFINITY : 0.f) + (down > 0.f ? -INFINITY : 0.f); }
+// the four values from `feature` on at a place, those that are not finite; 0 for the others
+__device__ __forceinline__ void special4(const uint16_t *v, float (&x)[4], bool seen) {
+  const uint2 w = *reinterpret_cast<const uint2 *>(v);
+  x[0] = special_of(__uint_as_float(w.x << 16), seen); x[1] = special_of(__uint_as_float(w.x & 0xffff0000u), seen);
+  x[2] = special_of(__uint_as_float(w.y << 16), seen); x[3] = special_of(__uint_as_float(w.y & 0xffff0000u), seen);
+}
 
 // ------------------------------------------------------------------------------------------ joining
 // The finished column: o and lse, or one unit's part of them.  m in units of `natural` (its logarithm's base), l the sum of weights.
@@ -259,6 +259,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 #pragma unroll
   for (int d = 0; d < DB; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+  bool specials = false;
 
   u32x4 kr[2][KS], vr[NV];
   auto load = [&](int32_t page, int base) {        // a tile's rows: lane r (and r + 32) looks after position base + r
@@ -337,38 +338,43 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
         l += w;
         p[4 * h + r] = (__bf16)w;
       }
-    auto values = [&](int d) {
-      const uint16_t *at = tile + (4 * g + (col >> 2)) * G::PITCH + 16 * d + 4 * (col & 3);
+    auto values = [&](const uint16_t *from, int d) {
+      const uint16_t *at = from + (4 * g + (col >> 2)) * G::PITCH + 16 * d + 4 * (col & 3);
       const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(at + 16 * G::PITCH));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     bool special = false;
     if (edge && least < end) {                                       // some columns see less than others
       keep_branch();
-#pragma unroll
-      for (int d = 0; d < DB; d++) special |= has_special(values(d));
+#pragma unroll 1
+      for (int d = 0; d < DB; d++) special |= has_special(values((const uint16_t *)apart((const char *)tile), d));
       special = __any(special);
+      specials |= special;
     }
     if (!special) {
 #pragma unroll
-      for (int d = 0; d < DB; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), p, o[d], 0, 0, 0);
+      for (int d = 0; d < DB; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(tile, d), p, o[d], 0, 0, 0);
     } else {
-      const bf16x8 seen_p = ones_where_seen(p);
-      for (int d = 0; d < DB; d++) {
-        bf16x8 rest, up, down;
-        take_special(values(d), rest, up, down);
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const f32x4 ups = __builtin_amdgcn_mfma_f32_16x16x32_bf16(up, seen_p, zero, 0, 0, 0), downs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(down, seen_p, zero, 0, 0, 0);
-        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+      const uint16_t *again = (const uint16_t *)apart((const char *)tile);
 #pragma unroll
-        for (int e = 0; e < DB; e++) x = e == d ? o[e] : x;
-        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rest, p, x, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; r++) x[r] = put_back(x[r], ups[r], downs[r]);
-#pragma unroll
-        for (int e = 0; e < DB; e++) o[e] = e == d ? x : o[e];
-      }
+      for (int d = 0; d < DB; d++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(finite_of(values(again, d)), p, o[d], 0, 0, 0);
     }
+  }
+  if (specials) {
+    keep_branch();
+    for (int b = begin + wave * 32; b < end; b += stride)
+      for (int kv = b; b + 32 > least && kv < min(b + 32, end); kv++) {
+        const int64_t at = position_place(a.c, u.seq, kv);
+        if (at < 0) continue;
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+          if (16 * d + 4 * g >= a.head_dim) continue;
+          float x[4];
+          special4(V + at + 16 * d + 4 * g, x, kv < limit);
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[d][r] += x[r];
+        }
+      }
   }
 
   // the four waves: weights relative to the largest of their maxima
@@ -410,35 +416,47 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------ rows, bf16
-// Four waves of 32 columns on v_mfma_f32_32x32x16_bf16, K and V in LDS in tiles of 64 positions, two of them in turn (one barrier to a tile), the next tile's
-// rows on their way in registers and the table's entries for the one behind that.  MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself
-// for the maximum (attention_bf16.hip); 2: a larger cap.
-template <int D>
-struct RowsPlaces {                                  // where this thread's pieces of a tile lie
-  static constexpr int N = Geo<D>::CHUNKS;
-  static __device__ __forceinline__ int row(int n) { return (threadIdx.x + 256 * n) / (D / 8); }
-  static __device__ __forceinline__ int feature() { return threadIdx.x % (D / 8) * 8; }
+// Four waves of 32 columns on v_mfma_f32_32x32x16_bf16 (operands as in attention_bf16.hip), K and V in LDS in tiles of 64 positions, two of them in turn,
+// one barrier to a tile.  The tiles come by global_load_lds, 16 bytes to a lane from wherever its position's page lies, past the registers; what does not
+// exist is fetched from rows of zeros or NaN.  A wave's 1 KB lands in lane order, so rows cannot be padded: the 16-byte pieces of a row are permuted instead
+// (by the lane that fetches them), so that 16 rows' same piece and four rows' same 64 bytes each meet all 64 banks.
+// MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself for the maximum (attention_bf16.hip); 2: a larger cap.
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
+__device__ __attribute__((aligned(16))) const uint32_t nothing[2][4] = {{0u, 0u, 0u, 0u}, {NAN_PAIR, NAN_PAIR, NAN_PAIR, NAN_PAIR}};
+
+template <int D> struct RowsTile {
+  static constexpr int PIECES = D / 8, ROW = 2 * D, BYTES = ST * ROW;         // 16-byte pieces of a row, bytes
+  static constexpr int LOADS = ST * PIECES / 256;                             // of a wave for K, and for V
+  static __device__ __forceinline__ int turned(int row) {                     // what a row's piece numbers are XORed with
+    if constexpr (PIECES == 16) return (row & 3) << 2 | (row >> 2 & 3);
+    else if constexpr (PIECES == 8) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    else return row >> 2 & 3;
+  }
 };
 
 template <int D, int MODE>
-__device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
-  constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = RowsPlaces<D>::N;
+__global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
+  using G = RowsTile<D>;
+  constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = G::LOADS;
   constexpr bool CAPPED = MODE == 1;
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[2][Geo<D>::ELEMS], Vs[2][Geo<D>::ELEMS];
+  __shared__ __attribute__((aligned(1024))) char Ks[2][G::BYTES], Vs[2][G::BYTES];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
   const int head = blockIdx.x % a.kv_heads;
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
   const int columns = u.s.count * a.group, i0 = u.tile * TILE + wave * 32, i = i0 + lr;
-  const int limit = i < columns ? u.limit(i, a.group) : 0;
   const int last = min((u.tile + 1) * TILE, columns) - 1, wave_last = min(i0 + 31, columns - 1);
   const int begin = u.parts > 1 ? u.part * u.span : 0;
   const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
   const int wave_end = wave_last < i0 ? 0 : min(u.limit(wave_last, a.group), end), least = u.limit(min(i0, columns - 1), a.group);
+  const int limit = i < columns ? min(u.limit(i, a.group), end) : 0;          // positions that the column sees of these
   const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
   const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
-  const float c1 = (MODE ? 2.0f * a.scale * LOG2E / a.cap : a.scale * LOG2E), c2 = a.cap * LOG2E;
-  const float ic2 = MODE ? -1.0f / (2.0f * c2) : 0.f;                // p = 2^(-2 c2 r) and -2 c2 r = 1 / ((e + 1) ic2)
+  // MODE 0: the score in base 2 is c1 s, c1 >= 0 (a negative scale turns q's sign).  Capped: e^(2 x / cap) = 2^(c1 s), the score is c2 - 2 c2 / (that + 1)
+  const float c1 = (MODE ? 2.0f * a.scale / a.cap : fabsf(a.scale)) * LOG2E, c2 = a.cap * LOG2E;
+  const float ic2 = MODE ? -1.0f / (2.0f * c2) : 0.f;                         // and 2^(-2 c2 r) with -2 c2 r = 1 / ((e + 1) ic2)
+  const float slope = MODE ? 1.f : c1;
 
   bf16x8 qf[KS];
   const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
@@ -446,6 +464,7 @@ __device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
   for (int ks = 0; ks < KS; ks++) {
     u32x4 x = {0u, 0u, 0u, 0u};
     if (i < columns && ks * 16 + lk * 8 < a.head_dim) x = *reinterpret_cast<const u32x4 *>((const uint16_t *)a.q + row * a.q_st + h * a.q_sh + ks * 16 + lk * 8);
+    if (MODE == 0 && a.scale < 0.f) x ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
     qf[ks] = __builtin_bit_cast(bf16x8, x);
   }
   f32x16 o[DB];
@@ -454,44 +473,59 @@ __device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
 #pragma unroll
     for (int e = 0; e < 16; e++) o[d][e] = 0.f;
   float m = CAPPED ? c2 : -INFINITY, l = 0.f;
+  bool specials = false;
 
-  u32x4 rk[N], rv[N];
+  // what this lane fetches: piece `lane % PIECES` as it lands of row base + its_row(n)
+  auto its_row = [&](int n) { return (wave * N + n) * (64 / G::PIECES) + lane / G::PIECES; };
   int32_t entry[N];
-  const int feature = RowsPlaces<D>::feature();
-  const bool inside = feature < a.head_dim;
   auto entries = [&](int base) {
 #pragma unroll
-    for (int n = 0; n < N; n++) entry[n] = page_entry(a.c, table, base + RowsPlaces<D>::row(n), end);
+    for (int n = 0; n < N; n++) entry[n] = page_entry(a.c, table, base + its_row(n), end);
   };
-  auto load = [&](int base) {
+  auto load = [&](int buf, int base) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int64_t at = place_of(a.c, entry[n], base + RowsPlaces<D>::row(n), end);
-      rk[n] = piece_or(K, at, feature, inside, NAN_PAIR);
-      rv[n] = piece_or(V, at, feature, inside, 0u);
+      const int r = its_row(n), feature = (lane % G::PIECES ^ G::turned(r)) * 8;
+      const int64_t at = place_of(a.c, entry[n], base + r, end);
+      const bool here = at >= 0 && feature < a.head_dim;
+      const uint16_t *k = here ? K + at + feature : (const uint16_t *)nothing[at == NO_PAGE && feature < a.head_dim], *v = here ? V + at + feature : (const uint16_t *)nothing[0];
+      __builtin_amdgcn_global_load_lds((glb_void *)k, (lds_void *)(Ks[buf] + (wave * N + n) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void *)v, (lds_void *)(Vs[buf] + (wave * N + n) * 1024), 16, 0, 0);
     }
   };
+  const int k_turned = G::turned(lr);
+  auto keys = [&](const char *tile, int sub, int ks) {             // A operand: row sub + lr, features 16 ks + 8 lk ..
+    return *reinterpret_cast<const bf16x8 *>(tile + (sub + lr) * G::ROW + ((2 * ks + lk) ^ k_turned) * 16);
+  };
+  const int vj = lane & 15, vg = lane >> 4, v_row = 4 * (vg >> 1) + (vj >> 2), v_piece = 2 * (vg & 1) + (vj >> 1 & 1);
+  const int v_turned = G::turned(v_row), v_turned8 = G::turned(v_row + 8);
+  auto values = [&](const char *tile, int sub, int m_, int d) {    // A operand: feature 32 d + lane % 32, k-slot i row sub + 16 m + 8 (i / 4) + 4 lk + i % 4
+    const char *at = tile + (sub + 16 * m_ + v_row) * G::ROW + (vj & 1) * 8;
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(at + ((4 * d + v_piece) ^ v_turned) * 16));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(at + 8 * G::ROW + ((4 * d + v_piece) ^ v_turned8) * 16));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
   entries(begin);
-  load(begin);
+  load(0, begin);
   entries(begin + ST);
-  tile_store<D>(Ks[0], rk);
-  tile_store<D>(Vs[0], rv);
-  __syncthreads();
   int cur = 0;
   for (int base = begin; base < end; base += ST, cur ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // this tile is there, for all behind the barrier
+    __syncthreads();
     if (base + ST < end) {
-      load(base + ST);
+      load(cur ^ 1, base + ST);
       entries(base + 2 * ST);
     }
-#pragma unroll
-    for (int sub = 0; sub < ST / 32; sub++) {
-      const int kv0 = base + sub * 32;
-      if (kv0 >= wave_end) continue;                                 // (the same for the wave) nothing for its columns
+    const char *kt = Ks[cur], *vt = Vs[cur];
+#pragma unroll 1
+    for (int sub = 0; sub < ST; sub += 32) {
+      const int kv0 = base + sub;
+      if (kv0 >= wave_end) break;                                  // (the same for the wave) nothing for its columns
       f32x16 s;
 #pragma unroll
       for (int e = 0; e < 16; e++) s[e] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag<D>(Ks[cur], sub * 32, ks, lane), qf[ks], s, 0, 0, 0);
+      for (int ks = 0; ks < KS; ks++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(kt, sub, ks), qf[ks], s, 0, 0, 0);
       const bool edge = kv0 + 32 > min(least, end);
       if (MODE == 1) {
 #pragma unroll
@@ -499,24 +533,26 @@ __device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
         if (edge) {
           keep_branch();
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < min(limit, end) ? s[e] : 0.f;
+          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[e] : 0.f;
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) l += s[e];
       } else {
+        if (MODE == 2) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = MODE == 2 ? fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[e] * c1) + 1.0f), c2) : s[e] * c1;
+          for (int e = 0; e < 16; e++) s[e] = fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[e] * c1) + 1.0f), c2);
+        }
         if (edge) {
           keep_branch();
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < min(limit, end) ? s[e] : -INFINITY;
+          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[e] : -INFINITY;
         }
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
         top = max_lane<32>(top);
         if (__any(top > m)) {
-          const float larger = fmaxf(m, top), keep = exp2_fast(m - (larger == -INFINITY ? 0.f : larger));
+          const float larger = fmaxf(m, top), keep = exp2_fast((m - (larger == -INFINITY ? 0.f : larger)) * slope);
           l *= keep;
 #pragma unroll
           for (int d = 0; d < DB; d++)
@@ -524,53 +560,57 @@ __device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
             for (int e = 0; e < 16; e++) o[d][e] *= keep;
           m = larger;
         }
-        const float shift = m == -INFINITY ? 0.f : m;
+        const float shift = (m == -INFINITY ? 0.f : -m) * slope;
 #pragma unroll
-        for (int e = 0; e < 16; e++) { s[e] = exp2_fast(s[e] - shift); l += s[e]; }
+        for (int e = 0; e < 16; e++) { s[e] = exp2_fast(fmaf(s[e], slope, shift)); l += s[e]; }
       }
       const bf16x8 p0 = acc_to_b(s, 0), p1 = acc_to_b(s, 1);
       bool special = false;
-      if (edge && least < end) {                                     // some columns see less than others
+      if (edge && least < end) {                                   // some columns see less than others
         keep_branch();
-#pragma unroll
-        for (int d = 0; d < DB; d++) special |= has_special(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane)) | has_special(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane));
+        const char *again = apart(vt);
+#pragma unroll 1
+        for (int d = 0; d < DB; d++) special |= has_special(values(again, sub, 0, d)) | has_special(values(again, sub, 1, d));
         special = __any(special);
       }
       if (!special) {
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane), p0, o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane), p1, o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 0, d), p0, o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 1, d), p1, o[d], 0, 0, 0);
         }
       } else {
-        const bf16x8 seen0 = ones_where_seen(p0), seen1 = ones_where_seen(p1);
+        specials = true;
+        const char *again = apart(vt);
 #pragma unroll
         for (int d = 0; d < DB; d++) {
-          f32x16 ups, downs;
-#pragma unroll
-          for (int e = 0; e < 16; e++) { ups[e] = 0.f; downs[e] = 0.f; }
-          bf16x8 rest, up, down;
-          take_special(tile_frag_t<D>(Vs[cur], sub * 32, 0, d, lane), rest, up, down);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, p0, o[d], 0, 0, 0);
-          ups = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen0, ups, 0, 0, 0);
-          downs = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen0, downs, 0, 0, 0);
-          take_special(tile_frag_t<D>(Vs[cur], sub * 32, 1, d, lane), rest, up, down);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest, p1, o[d], 0, 0, 0);
-          ups = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen1, ups, 0, 0, 0);
-          downs = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen1, downs, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 16; e++) o[d][e] = put_back(o[d][e], ups[e], downs[e]);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_of(values(again, sub, 0, d)), p0, o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_of(values(again, sub, 1, d)), p1, o[d], 0, 0, 0);
         }
       }
     }
-    if (base + ST < end) {
-      tile_store<D>(Ks[cur ^ 1], rk);
-      tile_store<D>(Vs[cur ^ 1], rv);
+  }
+  if (specials) {
+    keep_branch();
+    for (int kv = least > begin ? begin + (least - begin) / 32 * 32 : begin; kv < wave_end; kv++) {
+      const int64_t at = position_place(a.c, u.seq, kv);
+      if (at < 0) continue;
+#pragma unroll
+      for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          asm volatile("" ::: "memory");                           // (one after the other: few registers)
+          if (32 * d + 8 * j + 4 * lk >= a.head_dim) continue;
+          float x[4];
+          special4(V + at + 32 * d + 8 * j + 4 * lk, x, kv < limit);
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[d][4 * j + r] += x[r];
+        }
     }
-    __syncthreads();
   }
   l = add_lane<32>(l);
   if (CAPPED && l == 0.f) m = -INFINITY;
+  if (MODE == 0 && m > -INFINITY) m *= c1;                           // (to base 2)
   if (i >= columns) return;
   if (u.parts > 1) {
     float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
@@ -583,12 +623,10 @@ __device__ __forceinline__ void paged_rows_bf16_body(const AttendArgs &a) {
     if (lk == 0) { part[TILE * D + c] = m; part[TILE * D + TILE + c] = l; }
     return;
   }
-  l = column_sum(l, limit, a.c.capacity);
+  l = column_sum(l, u.limit(i, a.group), a.c.capacity);
   store_rows<D, true>((uint16_t *)a.o + row * a.o_st + h * a.o_sh, o, l == 0.f ? 0.f : 1.0f / l, lane, a.head_dim);
   if (lk == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
 }
-template <int D, int MODE>
-__global__ __launch_bounds__(256, D <= 32 ? 3 : D <= 64 ? 2 : 1) void k_paged_rows_bf16(AttendArgs a) { paged_rows_bf16_body<D, MODE>(a); }
 
 // ------------------------------------------------------------------------------------------ fp32
 // v_mfma_f32_16x16x4_f32, nothing through LDS before the end: a tile is 16 positions, S^T[16 positions, 16 columns] = K Q^T, whose slot g of
@@ -639,6 +677,7 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
     l[n] = 0.f;
   }
 
+  bool specials = false;
   f32x4 kr[KQ];
   float vr[4][VH][W];
   auto load = [&](int32_t page, int base) {           // lane l looks after position base + l % 16
@@ -696,7 +735,15 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
         for (int h = 0; h < VH; h++)
 #pragma unroll
           for (int c = 0; c < W; c++) special |= !(fabsf(v[r][h][c]) < INFINITY);
-      special = __any(special);
+      if (__any(special)) {
+        specials = true;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int h = 0; h < VH; h++)
+#pragma unroll
+            for (int c = 0; c < W; c++) v[r][h][c] = fabsf(v[r][h][c]) < INFINITY ? v[r][h][c] : 0.f;
+      }
     }
 #pragma unroll
     for (int n = 0; n < NC; n++) {
@@ -730,32 +777,34 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
       const float shift = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
       for (int r = 0; r < 4; r++) { s[r] = exp2_fast((s[r] - shift) * LOG2E); l[n] += s[r]; }
-      if (!special) {
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int h = 0; h < VH; h++)
-#pragma unroll
-            for (int c = 0; c < W; c++) o[n][W * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][h][c], s[r], o[n][W * h + c], 0, 0, 0);
-      } else {
+      for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int h = 0; h < VH; h++)
 #pragma unroll
-          for (int c = 0; c < W; c++) {
-            f32x4 ups = {0.f, 0.f, 0.f, 0.f}, downs = {0.f, 0.f, 0.f, 0.f};
+          for (int c = 0; c < W; c++) o[n][W * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][h][c], s[r], o[n][W * h + c], 0, 0, 0);
+    }
+  }
+  if (specials) {
+    keep_branch();
+    for (int b = begin + (SPLIT ? wave * 16 : 0); b < wave_end; b += stride)
+      for (int kv = b; b + 16 > least && kv < min(b + 16, wave_end); kv++) {
+        const int64_t at = position_place(a.c, u.seq, kv);
+        if (at < 0) continue;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const float x = v[r][h][c], one = s[r] == 0.f ? 0.f : 1.f;
-              const bool fine = fabsf(x) < INFINITY;
-              o[n][W * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(fine ? x : 0.f, s[r], o[n][W * h + c], 0, 0, 0);
-              ups = __builtin_amdgcn_mfma_f32_16x16x4f32(!fine && !(x < 0.f) ? 1.f : 0.f, one, ups, 0, 0, 0);
-              downs = __builtin_amdgcn_mfma_f32_16x16x4f32(!fine && !(x > 0.f) ? 1.f : 0.f, one, downs, 0, 0, 0);
+        for (int h = 0; h < VH; h++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int f = W * (16 * h + 4 * g + r);
+            if (f >= a.head_dim) continue;
+#pragma unroll
+            for (int c = 0; c < W; c++) {
+              const float x = V[at + f + c];
+#pragma unroll
+              for (int n = 0; n < NC; n++) o[n][W * h + c][r] += special_of(x, kv < limit[n]);
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++) o[n][W * h + c][r] = put_back(o[n][W * h + c][r], ups[r], downs[r]);
           }
       }
-    }
   }
   // a lane has features W (16 h + 4 g + r) + c of its column in element r of block W h + c
   if constexpr (!SPLIT) {
