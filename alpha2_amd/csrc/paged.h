@@ -30,6 +30,7 @@ constexpr int32_t MOST_POSITIONS = 0x7fff0000;      // so that a tile behind a p
 struct PagedCache {
   const int32_t *table, *starts, *lens;
   int64_t  pages, page_stride, row_stride, head_stride;
+  uint32_t page_pieces, row_pieces;      // strides of a page and of a row in 16 bytes
   Quotient page_rows;
   int32_t  seqs, table_pages;
   int32_t  rows;              // of the arrays of new tokens

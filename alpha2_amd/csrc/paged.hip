@@ -19,12 +19,13 @@ int32_t paged_cache(const char *who, const AhPages *p, int32_t rows, PagedCache 
   AH_ARG(p->page_stride % piece == 0 && p->row_stride % piece == 0 && p->head_stride % piece == 0, "%s: page strides of whole 16 bytes, got %lld, %lld, %lld", who,
          (long long)p->page_stride, (long long)p->row_stride, (long long)p->head_stride);
   AH_ARG(p->page_stride >= 0 && p->row_stride >= 0 && p->head_stride >= 0, "%s: page strides are not negative", who);
+  AH_ARG(p->page_stride / piece <= INT32_MAX && p->row_stride / piece <= INT32_MAX && p->head_stride / piece <= INT32_MAX, "%s: page strides of 2^31 times 16 bytes and more", who);
   AH_ARG(aligned16(p->k) && aligned16(p->v) && p->table % 4 == 0 && p->starts % 4 == 0 && p->lens % 4 == 0, "%s: pages that are not 16-byte aligned", who);
   if (rows > 0 && p->seqs > 0)
     AH_ARG(p->starts && p->lens && ((p->k && p->v && p->table) || p->pages == 0 || p->table_pages == 0), "%s: a null page array, table, starts or lens", who);
   const int64_t capacity = p->pages == 0 ? 0 : (int64_t)p->table_pages * p->page_rows;
   *out = PagedCache{dp<const int32_t>(p->table), dp<const int32_t>(p->starts), dp<const int32_t>(p->lens), p->pages, p->page_stride, p->row_stride, p->head_stride,
-                    quotient_by((uint32_t)p->page_rows), p->seqs, p->table_pages, rows, (int32_t)(capacity < MOST_POSITIONS ? capacity : MOST_POSITIONS)};
+                    (uint32_t)(p->page_stride / piece), (uint32_t)(p->row_stride / piece), quotient_by((uint32_t)p->page_rows), p->seqs, p->table_pages, rows, (int32_t)(capacity < MOST_POSITIONS ? capacity : MOST_POSITIONS)};
   return AH_OK;
 }
 

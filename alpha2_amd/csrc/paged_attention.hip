@@ -475,20 +475,29 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   float m = CAPPED ? c2 : -INFINITY, l = 0.f;
   bool specials = false;
 
-  // what this lane fetches: piece `lane % PIECES` as it lands of row base + its_row(n)
+  // What this lane fetches: piece `lane % PIECES`, as it lands, of row base + its_row(n).  Positions past the end look at the last one's entry, so that nothing
+  // here branches: page and row in 16-byte pieces, one multiplication each, and the row of zeros or NaN where they name no place.
   auto its_row = [&](int n) { return (wave * N + n) * (64 / G::PIECES) + lane / G::PIECES; };
-  int32_t entry[N];
+  uint32_t entry[N], line[N];
   auto entries = [&](int base) {
 #pragma unroll
-    for (int n = 0; n < N; n++) entry[n] = page_entry(a.c, table, base + its_row(n), end);
+    for (int n = 0; n < N; n++) {
+      const uint32_t p = (uint32_t)min(base + its_row(n), end - 1), page = quotient(p, a.c.page_rows);
+      entry[n] = (uint32_t)table[page];
+      line[n] = p - page * a.c.page_rows.divisor;
+    }
   };
+  const uint32_t pages = (uint32_t)a.c.pages;
   auto load = [&](int buf, int base) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
-      const int r = its_row(n), feature = (lane % G::PIECES ^ G::turned(r)) * 8;
-      const int64_t at = place_of(a.c, entry[n], base + r, end);
-      const bool here = at >= 0 && feature < a.head_dim;
-      const uint16_t *k = here ? K + at + feature : (const uint16_t *)nothing[at == NO_PAGE && feature < a.head_dim], *v = here ? V + at + feature : (const uint16_t *)nothing[0];
+      const int r = its_row(n);
+      const uint32_t piece = (uint32_t)(lane % G::PIECES ^ G::turned(r));
+      const uint64_t at = (uint64_t)entry[n] * a.c.page_pieces + ((uint64_t)line[n] * a.c.row_pieces + piece);
+      const bool wanted = base + r < end && (int)piece * 8 < a.head_dim, there = entry[n] < pages;
+      const uint16_t *k = (const uint16_t *)nothing[0], *v = k;
+      k = wanted ? there ? K + at * 8 : (const uint16_t *)nothing[1] : k;
+      v = wanted && there ? V + at * 8 : v;
       __builtin_amdgcn_global_load_lds((glb_void *)k, (lds_void *)(Ks[buf] + (wave * N + n) * 1024), 16, 0, 0);
       __builtin_amdgcn_global_load_lds((glb_void *)v, (lds_void *)(Vs[buf] + (wave * N + n) * 1024), 16, 0, 0);
     }
@@ -505,9 +514,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(at + 8 * G::ROW + ((4 * d + v_piece) ^ v_turned8) * 16));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  entries(begin);
-  load(0, begin);
-  entries(begin + ST);
+  if (begin < end) {
+    entries(begin);
+    load(0, begin);
+    entries(begin + ST);
+  }
   int cur = 0;
   for (int base = begin; base < end; base += ST, cur ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // this tile is there, for all behind the barrier

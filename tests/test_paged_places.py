@@ -103,7 +103,7 @@ BAD_PAGES = [(dict(dtype=ffi.F16), "dtype"), (dict(dtype=9), "dtype"), (dict(kv_
              (dict(head_dim=0), "head_dim"), (dict(head_dim=60), "head_dim"), (dict(head_dim=136), "head_dim"), (dict(page_rows=0), "page_rows"),
              (dict(page_rows=65537), "page_rows"), (dict(seqs=-1), "sequences"), (dict(seqs=1 << 21), "sequences"), (dict(table_pages=-1), "pages"),
              (dict(pages=-1), "pages"), (dict(pages=1 << 31), "pages"), (dict(page_stride=2044), "strides"), (dict(row_stride=132), "strides"),
-             (dict(head_stride=1), "strides"), (dict(head_stride=-64), "strides"), (dict(k=P + 8), "aligned"), (dict(v=P + 2), "aligned"),
+             (dict(head_stride=1), "strides"), (dict(head_stride=-64), "strides"), (dict(page_stride=1 << 35), "strides"), (dict(k=P + 8), "aligned"), (dict(v=P + 2), "aligned"),
              (dict(table=P + 2), "aligned"), (dict(lens=P + 1), "aligned"), (dict(starts=0), "null"), (dict(lens=0), "null"), (dict(k=0), "null"),
              (dict(v=0), "null"), (dict(table=0), "null")]
 
