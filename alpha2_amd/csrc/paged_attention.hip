@@ -46,7 +46,8 @@ struct Unit {
   Sequence s;
   int32_t seq, tile;          // -1: no such unit
   int32_t part, parts;        // parts that hold positions which a column of the tile sees (at least one)
-  int32_t span;               // positions of a part
+  int32_t span;               // positions of a part, at most: the launch's
+  int32_t own;                // and this sequence's, whose parts are as long as each other
   int32_t first;              // the tile's first unit
   // the positions that column `i` of the sequence sees
   __device__ __forceinline__ int limit(int i, int group) const { return s.len - s.count + i / group + 1; }
@@ -97,7 +98,9 @@ __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan,
       u.first = by_tile ? 0 : before + t * p;
       const int last = min((u.tile + 1) * TILE, u.s.count * group) - 1;
       const int seen = min(u.limit(last, group), c.capacity);
-      u.parts = parts_of(seen, u.span);
+      const int reach = min(u.s.len, c.capacity);
+      u.own = p > 1 ? ((reach - 1) / p + 64) / 64 * 64 : u.span;     // (at most span, a multiple of 64 as well)
+      u.parts = parts_of(seen, u.own);
       // (by tile, the units before it are those of all tiles before it)
       if (by_tile) u.first = t * p;
       break;
@@ -171,13 +174,19 @@ template <> __device__ __forceinline__ void store4<uint16_t>(uint16_t *p, float 
 }
 constexpr float LN2 = 0.693147180559945309f;
 
-// Joins the parts of a tile: a workgroup to a tile and kv head, a thread to four features of a column.  Maxima are logarithms to base 2.
+constexpr int join_slices(int tile, int d) { return tile * d / 4 > 256 ? tile * d / 4 / 256 : 1; }
+// Joins the parts of a tile: a thread to four features of a column, a workgroup to 256 such of a tile and kv head (a workgroup to all 128 columns of a
+// tile has too few of them at work: at 4 sequences of 8 kv heads in 16 parts, 32 columns each, 63 us against 39).  Maxima are logarithms to base 2.
 template <class T, int TILE, int D>
 __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
-  const int head = blockIdx.x % a.kv_heads;
+  constexpr int SLICES = join_slices(TILE, D);
+  const int index = blockIdx.x / SLICES, head = index % a.kv_heads;
   // the units of the tiles before this one have to be known: find_unit by tile gives those of the sequence, the others are added up here
-  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, true);
+  const Unit u = find_unit<TILE>(a.c, a.plan, a.group, index / a.kv_heads, true);
   if (u.seq < 0 || u.parts == 1) return;
+  const int e = blockIdx.x % SLICES * 256 + threadIdx.x, col = e / (D / 4), f = e % (D / 4) * 4, i = u.tile * TILE + col;
+  const int columns = u.s.count * a.group;
+  if (u.tile * TILE + (int)(blockIdx.x % SLICES) * 256 / (D / 4) >= columns) return;          // (all of it)
   int before = 0;
   for (int s0 = 0; s0 < u.seq; s0 += 64) {
     const int s = s0 + (threadIdx.x & 63);
@@ -189,28 +198,27 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
   const int64_t first = before + u.first;
-  const int columns = u.s.count * a.group;
-  for (int e = threadIdx.x; e < TILE * D / 4; e += 256) {
-    const int col = e / (D / 4), f = e % (D / 4) * 4, i = u.tile * TILE + col;
-    if (i >= columns || f >= a.head_dim) continue;
-    float m = -INFINITY;
-    for (int p = 0; p < u.parts; p++) m = fmaxf(m, part_at<TILE, D>(a.plan, (first + p) * a.kv_heads + head)[TILE * D + col]);
-    const float shift = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < u.parts; p++) {
-      const float *part = part_at<TILE, D>(a.plan, (first + p) * a.kv_heads + head);
-      const float w = exp2_fast(part[TILE * D + col] - shift);
-      const float4 x = *reinterpret_cast<const float4 *>(part + col * D + f);
-      l = fmaf(part[TILE * D + TILE + col], w, l);
-      o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
-    }
-    l = column_sum(l, u.limit(i, a.group), a.c.capacity);
-    const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    store4<T>((T *)a.o + row * a.o_st + h * a.o_sh + f, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (f == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
+  if (i >= columns || col >= TILE || f >= a.head_dim) return;
+  const int64_t pitch = (int64_t)a.kv_heads * (TILE * (D + 2));
+  const float *part = part_at<TILE, D>(a.plan, first * a.kv_heads + head), *stats = part + TILE * D + col;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < u.parts; p++) m = fmaxf(m, stats[p * pitch]);
+  const float shift = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int p = 0; p < u.parts; p++) {
+    const float w = exp2_fast(stats[p * pitch] - shift);
+    const float4 x = *reinterpret_cast<const float4 *>(part + p * pitch + col * D + f);
+    l = fmaf(stats[p * pitch + TILE], w, l);
+    o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
   }
+  l = column_sum(l, u.limit(i, a.group), a.c.capacity);
+  const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  store4<T>((T *)a.o + row * a.o_st + h * a.o_sh + f, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (f == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
 }
 
 // ------------------------------------------------------------------------------------------ keys, bf16
@@ -236,8 +244,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
   const int columns = u.s.count * a.group, i = u.tile * TILE + col, last = min((u.tile + 1) * TILE, columns) - 1;
   const int limit = i < columns ? u.limit(i, a.group) : 0;
   const int least = u.limit(u.tile * TILE, a.group);                 // every column sees the positions before this one
-  const int begin = u.parts > 1 ? u.part * u.span : 0;
-  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
+  const int begin = u.parts > 1 ? u.part * u.own : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.own, seen) : seen;
   const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
   const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
   uint16_t *tile = (uint16_t *)(own + wave * G::WAVE_BYTES);
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 // MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself for the maximum (attention_bf16.hip); 2: a larger cap.
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
-__device__ __attribute__((aligned(16))) const uint32_t nothing[2][4] = {{0u, 0u, 0u, 0u}, {NAN_PAIR, NAN_PAIR, NAN_PAIR, NAN_PAIR}};
+__device__ __attribute__((aligned(16))) const uint32_t nothing[3][4] = {{0u, 0u, 0u, 0u}, {NAN_PAIR, NAN_PAIR, NAN_PAIR, NAN_PAIR}, {0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u}};      // (bf16, fp32)
 
 template <int D> struct RowsTile {
   static constexpr int PIECES = D / 8, ROW = 2 * D, BYTES = ST * ROW;         // 16-byte pieces of a row, bytes
@@ -447,8 +455,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
   const int columns = u.s.count * a.group, i0 = u.tile * TILE + wave * 32, i = i0 + lr;
   const int last = min((u.tile + 1) * TILE, columns) - 1, wave_last = min(i0 + 31, columns - 1);
-  const int begin = u.parts > 1 ? u.part * u.span : 0;
-  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
+  const int begin = u.parts > 1 ? u.part * u.own : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.own, seen) : seen;
   const int wave_end = wave_last < i0 ? 0 : min(u.limit(wave_last, a.group), end), least = u.limit(min(i0, columns - 1), a.group);
   const int limit = i < columns ? min(u.limit(i, a.group), end) : 0;          // positions that the column sees of these
   const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
@@ -644,27 +652,27 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // instruction (j, c) is taken to mean feature 16 j + 4 g + c, so that both operands are 16-byte loads; a lane then holds positions 4 g + r of column
 // lane % 16, the B operand of O^T += V^T P^T whose slot g of instruction r means that position, and the A operand's row n of block (h, c) is taken
 // to mean feature W (16 h + n) + c with W = min(4, D / 16), so that V's pieces are 16-byte loads (8 at D = 32) of whole rows too.
-// SPLIT: 16 columns, the waves take tiles in turn and are joined (keys).  Otherwise every wave has NC times 16 columns of its own and streams all
-// positions; what one wave reads the others find in the caches (rows).
+// The waves take tiles in turn and are joined, for NC = 1 block of columns (keys) and for 2 (rows): no wave waits for another before the end, and
+// each piece of a page is read once by a workgroup.  With 32 columns to a wave, each streaming all positions, a batch of prompts of 12 heads of 64
+// took 254 us; with the positions cut, 168, and with one block as long, but chunks of 512 in 4096 positions, 16 heads of 64: 398 us, two 369 (88 TFLOP/s of
+// the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.
 // a score through the cap: cap tanh(x), x = score / cap
 __device__ __forceinline__ float capped_f32(float x, float cap) { return cap * (fabsf(x) < TANH_SMALL ? tanh_small(x) : tanh_large(x)); }
 
-template <int D, int NC, bool SPLIT>
-__device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
-  constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = SPLIT ? 16 : 64 * NC, O_PITCH = D + 4;
-  static_assert(!SPLIT || NC == 1, "one block of columns where the waves share them");
-  __shared__ __attribute__((aligned(16))) float joined[SPLIT ? 4 * 16 * O_PITCH : 4];
-  __shared__ float tops[4][16], sums[4][16];
+template <int D, int NC>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
+  constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
+  __shared__ __attribute__((aligned(16))) float joined[4 * TILE * O_PITCH];
+  __shared__ float tops[4][TILE], sums[4][TILE];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % a.kv_heads;
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
-  const int columns = u.s.count * a.group, i0 = u.tile * TILE + (SPLIT ? 0 : wave * 16 * NC);
+  const int columns = u.s.count * a.group, i0 = u.tile * TILE;
   const int last = min((u.tile + 1) * TILE, columns) - 1;
-  const int begin = u.parts > 1 ? u.part * u.span : 0;
-  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.span, seen) : seen;
-  const int wave_last = SPLIT ? last : min(i0 + 16 * NC - 1, columns - 1);
-  const int wave_end = wave_last < i0 ? 0 : min(u.limit(wave_last, a.group), end), least = u.limit(min(i0, columns - 1), a.group);
+  const int begin = u.parts > 1 ? u.part * u.own : 0;
+  const int seen = min(u.limit(last, a.group), a.c.capacity), end = u.parts > 1 ? min(begin + u.own, seen) : seen;
+  const int least = u.limit(i0, a.group);
   const float *K = (const float *)a.k + head * a.c.head_stride, *V = (const float *)a.v + head * a.c.head_stride;
   const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
   const float factor = a.cap > 0.f ? a.scale / a.cap : a.scale;
@@ -691,36 +699,44 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
   bool specials = false;
   f32x4 kr[KQ];
   float vr[4][VH][W];
-  auto load = [&](int32_t page, int base) {           // lane l looks after position base + l % 16
-    const int64_t place = place_of(a.c, page, base + col, end);
+  // Lane l looks after position base + l % 16: the table's entry (past the end, the last one's) and the row in its page; no branches, as in the rows' kernel.
+  const uint32_t pages = (uint32_t)a.c.pages;
+  auto entry_at = [&](int base, uint32_t &line) {
+    const uint32_t p = (uint32_t)max(0, min(base + col, end - 1)), page = quotient(p, a.c.page_rows);
+    line = p - page * a.c.page_rows.divisor;
+    return end > 0 ? (uint32_t)table[page] : 0u;
+  };
+  auto load = [&](uint32_t page, uint32_t line, int base) {
+    const uint64_t at = (uint64_t)page * a.c.page_pieces + (uint64_t)line * a.c.row_pieces;
+    const bool wanted = base + col < end, there = page < pages;
+    const float *k = wanted && there ? K + at * 4 : (const float *)nothing[wanted ? 2 : 0];
+    const uint64_t place = wanted && there ? at : ~0ull;
 #pragma unroll
     for (int j = 0; j < KQ; j++) {
       const bool inside = 16 * j + 4 * g < a.head_dim;
-      const float other = place == NO_PAGE && inside ? NAN : 0.f;
-      kr[j] = f32x4{other, other, other, other};
-      if (place >= 0 && inside) kr[j] = *reinterpret_cast<const f32x4 *>(K + place + 16 * j + 4 * g);
+      const float *p = wanted && there ? k + 16 * j + 4 * g : k;
+      kr[j] = *reinterpret_cast<const f32x4 *>(inside ? p : (const float *)nothing[0]);
     }
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const int64_t at = __shfl(place, 4 * g + r);
+      const uint64_t row = __shfl(place, 4 * g + r);
 #pragma unroll
       for (int h = 0; h < VH; h++) {
         const int f = W * (16 * h + col);
         typedef __attribute__((ext_vector_type(W))) float piece;
-        piece x;
-#pragma unroll
-        for (int c = 0; c < W; c++) x[c] = 0.f;
-        if (at >= 0 && f < a.head_dim) x = *reinterpret_cast<const piece *>(V + at + f);
+        const piece x = *reinterpret_cast<const piece *>(row != ~0ull && f < a.head_dim ? V + row * 4 + f : (const float *)nothing[0]);
 #pragma unroll
         for (int c = 0; c < W; c++) vr[r][h][c] = x[c];
       }
     }
   };
-  const int stride = SPLIT ? 64 : 16;
-  int base = begin + (SPLIT ? wave * 16 : 0);
-  int32_t next = page_entry(a.c, table, base + stride + col, end);
-  if (base < wave_end) load(page_entry(a.c, table, base + col, end), base);
-  for (; base < wave_end; base += stride) {
+  int base = begin + wave * 16;
+  uint32_t line, next_line, next = entry_at(base + 64, next_line);
+  {
+    const uint32_t first = entry_at(base, line);
+    if (base < end) load(first, line, base);
+  }
+  for (; base < end; base += 64) {
     f32x4 k[KQ];
     float v[4][VH][W];
 #pragma unroll
@@ -731,10 +747,11 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
       for (int h = 0; h < VH; h++)
 #pragma unroll
         for (int c = 0; c < W; c++) v[r][h][c] = vr[r][h][c];
-    if (base + stride < wave_end) {
-      const int32_t page = next;
-      next = page_entry(a.c, table, base + 2 * stride + col, end);
-      load(page, base + stride);
+    if (base + 64 < end) {
+      const uint32_t page = next;
+      line = next_line;
+      next = entry_at(base + 128, next_line);
+      load(page, line, base + 64);
     }
     const bool edge = base + 16 > min(least, end);
     bool special = false;
@@ -798,8 +815,8 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
   }
   if (specials) {
     keep_branch();
-    for (int b = begin + (SPLIT ? wave * 16 : 0); b < wave_end; b += stride)
-      for (int kv = b; b + 16 > least && kv < min(b + 16, wave_end); kv++) {
+    for (int b = begin + wave * 16; b < end; b += 64)
+      for (int kv = b; b + 16 > least && kv < min(b + 16, end); kv++) {
         const int64_t at = position_place(a.c, u.seq, kv);
         if (at < 0) continue;
 #pragma unroll
@@ -818,96 +835,65 @@ __device__ __forceinline__ void paged_f32_body(const AttendArgs &a) {
       }
   }
   // a lane has features W (16 h + 4 g + r) + c of its column in element r of block W h + c
-  if constexpr (!SPLIT) {
 #pragma unroll
-    for (int n = 0; n < NC; n++) {
-      const float sum = add_lane<16>(add_lane<32>(l[n]));
-      const int i = i0 + 16 * n + col;
-      if (i >= columns) continue;
-      float *to, mul = 1.f;
-      bool inside = true;
-      if (u.parts > 1) {
-        float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
-        const int c = wave * 16 * NC + 16 * n + col;
-        to = part + c * D;
-        if (g == 0) { part[TILE * D + c] = m[n] * LOG2E; part[TILE * D + TILE + c] = sum; }
-      } else {
-        const float all = column_sum(sum, u.limit(i, a.group), a.c.capacity);
-        const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
-        to = (float *)a.o + row * a.o_st + h * a.o_sh;
-        mul = all == 0.f ? 0.f : 1.0f / all;
-        inside = false;
-        if (g == 0 && a.lse) a.lse[row * a.heads + h] = all == 0.f ? -INFINITY : m[n] + logf(all);
-      }
+  for (int n = 0; n < NC; n++) {
+    const float mine = add_lane<16>(add_lane<32>(l[n]));
+    if (g == 0) { tops[wave][16 * n + col] = m[n]; sums[wave][16 * n + col] = mine; }
+  }
+  __syncthreads();
 #pragma unroll
-      for (int h = 0; h < VH; h++)
+  for (int n = 0; n < NC; n++) {
+    const int c0 = 16 * n + col;
+    const float top = fmaxf(fmaxf(tops[0][c0], tops[1][c0]), fmaxf(tops[2][c0], tops[3][c0]));
+    const float w = exp2_fast((m[n] - (top == -INFINITY ? 0.f : top)) * LOG2E);
+    float *to = joined + (wave * TILE + c0) * O_PITCH;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int f = W * (16 * h + 4 * g + r);
-          if (!inside && f >= a.head_dim) continue;
+    for (int h = 0; h < VH; h++)
 #pragma unroll
-          for (int c = 0; c < W; c += 2) *reinterpret_cast<float2 *>(to + f + c) = make_float2(o[n][W * h + c][r] * mul, o[n][W * h + c + 1][r] * mul);
-        }
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < W; c++) to[W * (16 * h + 4 * g + r) + c] = o[n][W * h + c][r] * w;
+  }
+  __syncthreads();
+  float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
+  for (int e = threadIdx.x; e < TILE * D / 4; e += 256) {
+    const int c = e / (D / 4), f = e % (D / 4) * 4, ci = u.tile * TILE + c;
+    if (ci >= columns || f >= a.head_dim) continue;
+    const float top = fmaxf(fmaxf(tops[0][c], tops[1][c]), fmaxf(tops[2][c], tops[3][c])), shift = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float4 y = *reinterpret_cast<const float4 *>(joined + (w * TILE + c) * O_PITCH + f);
+      sum = fmaf(sums[w][c], exp2_fast((tops[w][c] - shift) * LOG2E), sum);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-  } else {
-    const float mine = add_lane<16>(add_lane<32>(l[0]));
-    if (g == 0) { tops[wave][col] = m[0]; sums[wave][col] = mine; }
-    __syncthreads();
-    {
-      const float top = fmaxf(fmaxf(tops[0][col], tops[1][col]), fmaxf(tops[2][col], tops[3][col]));
-      const float w = exp2_fast((m[0] - (top == -INFINITY ? 0.f : top)) * LOG2E);
-      float *to = joined + (wave * 16 + col) * O_PITCH;
-#pragma unroll
-      for (int h = 0; h < VH; h++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int c = 0; c < W; c++) to[W * (16 * h + 4 * g + r) + c] = o[0][W * h + c][r] * w;
-    }
-    __syncthreads();
-    float *part = part_at<TILE, D>(a.plan, ((int64_t)u.first + u.part) * a.kv_heads + head);
-    for (int e = threadIdx.x; e < 16 * D / 4; e += 256) {
-      const int c = e / (D / 4), f = e % (D / 4) * 4, ci = u.tile * TILE + c;
-      if (ci >= columns || f >= a.head_dim) continue;
-      const float top = fmaxf(fmaxf(tops[0][c], tops[1][c]), fmaxf(tops[2][c], tops[3][c])), shift = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const float4 y = *reinterpret_cast<const float4 *>(joined + (w * 16 + c) * O_PITCH + f);
-        sum = fmaf(sums[w][c], exp2_fast((tops[w][c] - shift) * LOG2E), sum);
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
-      if (u.parts > 1) {
-        *reinterpret_cast<float4 *>(part + c * D + f) = x;
-        if (f == 0) { part[TILE * D + c] = top * LOG2E; part[TILE * D + TILE + c] = sum; }
-      } else {
-        sum = column_sum(sum, u.limit(ci, a.group), a.c.capacity);
-        const int64_t row = u.s.first + ci / a.group, h = (int64_t)head * a.group + ci % a.group;
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        store4<float>((float *)a.o + row * a.o_st + h * a.o_sh + f, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        if (f == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.f ? -INFINITY : top + logf(sum);
-      }
+    if (u.parts > 1) {
+      *reinterpret_cast<float4 *>(part + c * D + f) = x;
+      if (f == 0) { part[TILE * D + c] = top * LOG2E; part[TILE * D + TILE + c] = sum; }
+    } else {
+      sum = column_sum(sum, u.limit(ci, a.group), a.c.capacity);
+      const int64_t row = u.s.first + ci / a.group, h = (int64_t)head * a.group + ci % a.group;
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      store4<float>((float *)a.o + row * a.o_st + h * a.o_sh + f, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      if (f == 0 && a.lse) a.lse[row * a.heads + h] = sum == 0.f ? -INFINITY : top + logf(sum);
     }
   }
 }
-template <int D>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_keys_f32(AttendArgs a) { paged_f32_body<D, 1, true>(a); }
-template <int D>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_rows_f32(AttendArgs a) { paged_f32_body<D, 2, false>(a); }
-
 // ------------------------------------------------------------------------------------------ launches
 // Parts go through the library's scratch (64 MB from ah_init on, ordered with everything else on the main stream), of which a launch takes at most this.
 constexpr int64_t PART_BYTES = int64_t(60) << 20;
 
-// TILE columns to a unit: how many workgroups, and how many of them the positions are cut for.  `wanted` workgroups fill the GPU; where the tiles alone
-// are as many there is nothing to cut, and the join is not launched either where the table cannot name more positions than a part has.
+// TILE columns to a unit: how many workgroups, and how many of them the positions are cut for.  Two workgroups fit a compute unit; where the tiles alone
+// are as many, nothing is cut (64 sequences of 1024, 8 kv heads of 128, bf16: 44 us, 53 us cut), and the join is not launched either where the table
+// cannot name more positions than a part has.  Otherwise about `wanted` units are cut: more of them even out ragged sequences, fewer are fewer to join.
 template <class T, int TILE, int D, class Kernel>
 int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
   const int64_t tiles = cdiv((int64_t)a.c.rows * a.group, TILE) + a.c.seqs;                  // of one kv head, at most
   const int64_t slot = (int64_t)TILE * (D + 2) * sizeof(float) * a.kv_heads;
+  const int64_t cus = num_cus();
   int64_t target = 0;
-  if (tiles * a.kv_heads < wanted && a.c.capacity > least) {
+  if (tiles * a.kv_heads < 2 * cus && a.c.capacity > least) {
     target = cdiv(wanted, a.kv_heads);
     if ((tiles + target) * slot > PART_BYTES) target = PART_BYTES / slot - tiles;
     if (target < 1) target = 0;
@@ -923,21 +909,26 @@ int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
   launch_kernel(kernel, dim3((unsigned)grid), dim3(256), 0, a);
   AH_LAUNCH_CHECK();
   if (target > 0) {
-    launch_kernel(k_paged_join<T, TILE, D>, dim3((unsigned)(tiles * a.kv_heads)), dim3(256), 0, a);
+    launch_kernel(k_paged_join<T, TILE, D>, dim3((unsigned)(tiles * a.kv_heads * join_slices(TILE, D))), dim3(256), 0, a);
     AH_LAUNCH_CHECK();
   }
   return AH_OK;
 }
 template <int D>
 int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
-  const bool rows = (int64_t)a.c.rows * a.group > (int64_t)32 * a.c.seqs;                    // columns of a sequence, in the mean
+  // Columns of a sequence, in the mean.  At 32 the two are even (bf16, 4 x 8192 positions, 8 kv heads of 128: 40 and 39 us; fp32, 4 x 1024, 12 of 64: 19.0
+  // and 19.6); at 48, 60 and 44 us; at 256, 182 and 74.  The other way, 16 columns: 35 and 39 us.
+  const bool rows = (int64_t)a.c.rows * a.group > (int64_t)32 * a.c.seqs;
   const int64_t cus = num_cus();
+  // Units wanted, of keys: three to a compute unit, 246 us at 32 ragged sequences of up to 32768 positions; two, 277; four, 260.
+  // Least parts: of 128 positions in place of 256, one token after 256 positions takes 9.8 us, not 7.8 (bf16, 8 kv heads of 128), for the join; rows,
+  // whose units are longer, gain by it: 12 tokens after 512, 13.9 us against 18.7 with 256.
   if (bf16_pages) {
-    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 4 * cus, 256);
-    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 512);
+    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 3 * cus, 256);
+    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128);
   }
-  if (!rows) return attend<float, 16, D>(a, k_paged_keys_f32<D>, 4 * cus, 256);
-  return attend<float, 128, D>(a, k_paged_rows_f32<D>, 2 * cus, 512);
+  if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, 3 * cus, 256);
+  return attend<float, 32, D>(a, k_paged_f32<D, 2>, 3 * cus, 256);
 }
 
 }  // namespace
