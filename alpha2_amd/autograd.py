@@ -148,6 +148,7 @@ class Ctx:
     dropoutRng: Optional[DropoutRng] = None
     release: Release = None
     keptQkv: Optional[list] = None      # a list takes each block's q, k, v projection as it is computed
+    batch: Optional[object] = None      # decode.PagedContext: rows of several sequences, which attend to positions that it keeps
 
 
 def _record(ctx: Ctx, data: TensorData, inputs, backward, cleanup=None) -> Variable:

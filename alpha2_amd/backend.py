@@ -135,9 +135,28 @@ class TensorData:
         self._host_valid, self._dev_valid = True, False
 
 
+class Pages:
+    """Keys and values of many sequences in pages, and the batch of new tokens that is at them (AhPages): `k` and `v` are
+    [pages, positions to a page, heads, head size]; `table` [sequences, n] says which pages a sequence's positions lie in, in order,
+    `lens` [sequences] how many positions it has, the new ones among them, and `starts` [sequences + 1] where its new tokens' rows
+    begin (int32, all three).  The next batch, or the next token, is another Pages over the same k and v."""
+    __slots__ = ("k", "v", "table", "starts", "lens")
+
+    def __init__(self, k: TensorData, v: TensorData, table: TensorData, starts: TensorData, lens: TensorData):
+        if len(k.shape) != 4 or v.shape != k.shape or v.store != k.store:
+            raise ValueError(f"Pages: k {k.shape} {k.store} and v {v.shape} {v.store} must be [pages, positions, heads, head size] of one type")
+        if len(table.shape) != 2 or starts.shape != (table.shape[0] + 1,) or lens.shape != (table.shape[0],):
+            raise ValueError(f"Pages: table {table.shape}, starts {starts.shape} and lens {lens.shape} must be [sequences, n], [sequences + 1] and [sequences]")
+        for t in (table, starts, lens):
+            if t.dtype != "i32":
+                raise TypeError(f"Pages: table, starts and lens are i32, got {t.dtype}")
+        self.k, self.v, self.table, self.starts, self.lens = k, v, table, starts, lens
+
+
 class HipBackend:
     name = "hip"
     _timed: Optional[list] = None              # startTiming(): a record per product
+    activationStore = "f32"                    # how the projections that attention reads are stored
 
     def __init__(self, device: int = 0):
         self.lib = ffi.load()
@@ -965,6 +984,93 @@ class HipBackend:
         f.d_o, f.dq, f.dk, f.dv = self._ptr(dOut), dbase, dbase + Cc * esz, dbase + 2 * Cc * esz
         check(self.lib.ah_flash_bwd(C.byref(f)))
         return dqkv
+
+    # ------------------------------------------------------------------ many sequences at once (no counterpart in the reference)
+    def newPages(self, pages: int, positions: int, kvHeads: int, headDim: int, store: str = "f32"):
+        """Two tensors for Pages.k and Pages.v; what they hold is undefined, and read nowhere before it is written."""
+        return tuple(self._new((pages, positions, kvHeads, headDim), "f32", store) for _ in range(2))
+
+    def _stored(self, t: TensorData, store: str) -> TensorData:
+        if t.dtype != "f32" or t.store != store:
+            raise TypeError(f"op expects tensors of the pages' type {store}, got {t.dtype}/{t.store}")
+        return t
+
+    def _pages_desc(self, pages: Pages) -> ffi.AhPages:
+        n, positions, heads, D = pages.k.shape
+        p = ffi.AhPages()
+        p.dtype, p.kv_heads, p.head_dim, p.page_rows, p.pages = ffi.DTYPE_CODE[pages.k.store], heads, D, positions, n
+        p.seqs, p.table_pages = pages.table.shape
+        p.page_stride, p.row_stride, p.head_stride = positions * heads * D, heads * D, D
+        p.k, p.v = self._ptr(pages.k), self._ptr(pages.v)
+        p.table, p.starts, p.lens = self._ptr(pages.table), self._ptr(pages.starts), self._ptr(pages.lens)
+        return p
+
+    def pagedAppend(self, pages: Pages, qkv: TensorData, nHead: int, rotary: Optional[TensorData] = None, neighbours: bool = False) -> Optional[TensorData]:
+        """The new tokens' keys and values, of a fused projection [rows, (nHead + 2 heads of the pages) head size], go to their places.
+        With `rotary` [positions, n] (n / 2 cosines, then n / 2 sines, of every position) the first n features of queries and keys are
+        turned on the way, and the queries are returned, [rows, nHead head size]; without it the projection holds them as they are."""
+        heads, D = pages.k.shape[2:]
+        if len(qkv.shape) != 2 or nHead < 1 or qkv.shape[1] != (nHead + 2 * heads) * D:
+            raise ValueError(f"pagedAppend: qkv {qkv.shape} does not match {nHead} heads over {heads} in pages, of {D}")
+        if rotary is not None and len(rotary.shape) != 2:
+            raise ValueError(f"pagedAppend: rotary {rotary.shape} must be [positions, turned features]")
+        qkv = self._stored(qkv, pages.k.store)
+        for t in (pages.k, pages.v):
+            self._own(t)
+        p, a, base, esz = self._pages_desc(pages), ffi.AhPagedAppend(), self._ptr(qkv), ffi.DTYPE_BYTES[qkv.store]
+        a.rows, a.heads = qkv.shape[0], nHead
+        a.k, a.v = base + nHead * D * esz, base + (nHead + heads) * D * esz
+        a.q_st = a.k_st = a.v_st = qkv.shape[1]
+        a.q_sh = a.k_sh = a.v_sh = D
+        turned = None
+        if rotary is not None:
+            self._f32(rotary)
+            turned = self._new((qkv.shape[0], nHead * D), "f32", qkv.store)
+            a.rot_rows, a.rot_dim, a.rot_neighbours, a.rotary = *rotary.shape, int(neighbours), self._ptr(rotary)
+            a.q, a.rotated, a.r_st, a.r_sh = base, turned._buf.ptr, nHead * D, D
+        check(self.lib.ah_paged_append(C.byref(p), C.byref(a)))
+        self._dirty(pages.k)
+        self._dirty(pages.v)
+        return turned
+
+    def pagedAttention(self, pages: Pages, q: TensorData, nHead: int, scale: float, softCap: float = 0.0) -> dict:
+        """The new tokens attend to their sequences' positions up to their own: queries in the first nHead head size columns of q (what
+        pagedAppend returned, or the fused projection), output [rows, nHead head size], lse [rows, nHead].  Rows of no sequence are not
+        written.  Same function as attentionQkv of each sequence by itself."""
+        heads, D = pages.k.shape[2:]
+        if len(q.shape) != 2 or nHead < 1 or q.shape[1] < nHead * D:
+            raise ValueError(f"pagedAttention: q {q.shape} does not hold {nHead} heads of {D}")
+        q = self._stored(q, pages.k.store)
+        out, lse = self._new((q.shape[0], nHead * D), "f32", q.store), self._new((q.shape[0], nHead))
+        p, a = self._pages_desc(pages), ffi.AhPagedAttention()
+        a.rows, a.heads, a.scale, a.soft_cap = q.shape[0], nHead, scale, softCap
+        a.q_st, a.q_sh, a.o_st, a.o_sh = q.shape[1], D, nHead * D, D
+        a.q, a.o, a.lse = self._ptr(q), out._buf.ptr, lse._buf.ptr
+        check(self.lib.ah_paged_attention(C.byref(p), C.byref(a)))
+        return {"output": out, "lse": lse}
+
+    def sampleRows(self, logits: TensorData, uniform: TensorData, temperature: Optional[TensorData] = None, topk: Optional[TensorData] = None,
+                   topp: Optional[TensorData] = None, minp: Optional[TensorData] = None) -> dict:
+        """The next token behind each row of logits [rows, vocabulary], chosen as sample() does (sample.ts:85-193) with the row's own
+        random number in [0, 1) and its own options [rows] (None: temperature 1, no cut): tokens (i32) and the logarithms of their
+        probabilities, [rows] each."""
+        if len(logits.shape) != 2:
+            raise ValueError(f"sampleRows: logits {logits.shape} must be [rows, vocabulary]")
+        if logits.dtype != "f32":
+            raise TypeError(f"sampleRows: logits are f32, got {logits.dtype}")
+        rows, vocab = logits.shape
+        for name, t, dtype in (("uniform", uniform, "f32"), ("temperature", temperature, "f32"), ("topk", topk, "i32"), ("topp", topp, "f32"), ("minp", minp, "f32")):
+            if t is not None and t.shape != (rows,):
+                raise ValueError(f"sampleRows: {name} {t.shape} must be [{rows}]")
+            if t is not None and (t.dtype != dtype or t.store != dtype):
+                raise TypeError(f"sampleRows: {name} is {dtype}, got {t.dtype}/{t.store}")
+        tokens, logprobs = self._new((rows,), "i32"), self._new((rows,))
+        s = ffi.AhSample()
+        s.dtype, s.vocab, s.rows, s.ld, s.logits = ffi.DTYPE_CODE[logits.store], vocab, rows, vocab, self._ptr(logits)
+        s.uniform, s.temperature, s.top_k, s.top_p, s.min_p = (0 if t is None else self._ptr(t) for t in (uniform, temperature, topk, topp, minp))
+        s.tokens, s.logprobs = tokens._buf.ptr, logprobs._buf.ptr
+        check(self.lib.ah_sample(C.byref(s)))
+        return {"tokens": tokens, "logprobs": logprobs}
 
     # ------------------------------------------------------------------ reductions / optimizer
     def sumOfSquares(self, data: TensorData) -> TensorData:

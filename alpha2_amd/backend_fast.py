@@ -123,6 +123,7 @@ class _LazyTranspose:
 
 class FastHipBackend(HipBackend):
     name = "hip"
+    activationStore = "bf16"
     matmulTransposedGeluSaved = matmulGeluBackward = matmulTransposedAdd = None      # gelu, its backward and a residual join a product that is held back, whoever asks for the two
 
     def __init__(self, device: int = 0, group_weight_grads: bool = True, stream_bf16: bool = True, gelu_saves_derivative: bool = True):
@@ -233,6 +234,9 @@ class FastHipBackend(HipBackend):
     def _words(self, *ts):
         """Inherited data-movement kernels copy 4-byte elements: a bf16-stored tensor gets f32 storage first."""
         self._f32(*[t for t in ts if t.store == "bf16"])
+
+    def _stored(self, t: TensorData, store: str) -> TensorData:
+        return self.castStore(t, store) if t.dtype == "f32" else super()._stored(t, store)
 
     def _dirty(self, t: TensorData):
         super()._dirty(t)

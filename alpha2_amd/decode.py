@@ -1,21 +1,24 @@
-"""The logits behind a growing context, from kept keys and values.
+"""The logits behind a growing context, or several, from kept keys and values.
 
 Generation (packages/train/src/sample.ts:36-198) asks for the logits behind the last token of a context that grows by one token at
 a time, and the reference runs the forward pass over all of it each time.  Where every row attends to the rows before it through
 their keys and values alone (`attention == "heads"`, no dropout), those of earlier rows are what they were: the context is run once,
-its q, k, v projections are kept, and a token after that costs one row (ah_decode).  Same arithmetic, other orders of summation."""
+its q, k, v projections are kept, and a token after that costs one row (ah_decode).  Same arithmetic, other orders of summation.
+Several contexts of any lengths are one batch of rows (PagedContext): all but attention takes a row by itself, and attention finds a
+sequence's positions in pages (ah_paged_attention)."""
 from __future__ import annotations
 
 import ctypes
 import math
-from typing import Callable, Optional
+from typing import Callable, Optional, Sequence
 
 import numpy as np
 
 from . import _ffi as ffi
 from ._ffi import check
-from .autograd import Ctx, Tape
-from .backend import HipBackend, TensorData
+from . import autograd as ag
+from .autograd import Ctx, Tape, Variable
+from .backend import HipBackend, Pages, TensorData
 from .model import ModelConfig, ffn_dim, flashHeadSize, gptBlocks
 
 # bases of the MLP activations, as HipBackend.CHANNEL_BASES numbers them, and the parameter that holds each one's coefficients
@@ -136,3 +139,90 @@ class KeptContext:
             if t is not None:
                 self.backend.releaseGpuTensor(t)
         self.kv = self.logits = None
+
+
+class PagedContext:
+    """Several sequences: use `of`, then `forward` with the next tokens of any of them, then `close`.  The parameters' values must stay;
+    where they lie may change from call to call."""
+
+    PAGE = 64               # positions to a page
+    MOST_ROWS = 8192        # tokens of one pass that a caller should give it, for the memory that its activations take
+
+    @staticmethod
+    def of(cfg: ModelConfig, params: dict, backend, longest: Sequence[int]) -> Optional["PagedContext"]:
+        """For sequences of at most `longest` tokens each.  None where each has to be run by itself: another backend or wiring of
+        attention, a head size that the kernels do not take, or no memory for the keys and values."""
+        if not isinstance(backend, HipBackend) or cfg.attention != "heads" or cfg.dropout != 0:
+            return None
+        if cfg.nEmbd % cfg.nHead or not flashHeadSize(cfg.nEmbd // cfg.nHead) or cfg.vocabSize > 1 << 20 or max(longest) > cfg.blockSize:
+            return None
+        if params["wpe"].data.shape[0] < max(longest):
+            return None
+        kept = PagedContext(cfg, params, backend, longest)
+        try:
+            for _ in range(cfg.nLayer):
+                kept.layers.append(backend.newPages(kept.table[-1, -1] + 1, kept.PAGE, cfg.nHead, cfg.nEmbd // cfg.nHead, backend.activationStore))
+        except ffi.AlphaHipError:
+            kept.close()
+            return None
+        return kept
+
+    def __init__(self, cfg: ModelConfig, params: dict, backend: HipBackend, longest: Sequence[int]):
+        self.cfg, self.params, self.backend = cfg, params, backend
+        self.longest, self.lens = list(longest), np.zeros(len(longest), np.int64)
+        need = [-(-n // self.PAGE) for n in longest]
+        first = np.cumsum([0] + need[:-1])
+        # (entries behind a sequence's last page are not read)
+        self.table = np.array([np.minimum(f + np.arange(max(need)), f + n - 1) for f, n in zip(first, need)], np.int32)
+        self.layers, self._batch = [], (None, None, None)
+
+    def forward(self, seqs: Sequence[int], counts: Sequence[int], tokens, wanted: Sequence[int], releaseTensor: Optional[Callable]) -> Optional[TensorData]:
+        """`tokens`, the next counts[i] of sequence seqs[i] and so on (i32 in the host's memory, or a tensor), go through the model.  Logits
+        behind the last tokens of the i in `wanted`, [len(wanted), vocabulary]; None without any."""
+        B, cfg = self.backend, self.cfg
+        rows, lens = sum(counts), self.lens[list(seqs)] + counts
+        if len(set(seqs)) != len(seqs) or min(counts) < 1 or any(n > self.longest[i] for i, n in zip(seqs, lens)):
+            raise ValueError(f"{list(counts)} tokens more of sequences {list(seqs)}, which have {self.lens[list(seqs)]} of {[self.longest[i] for i in seqs]}")
+        if isinstance(tokens, TensorData):
+            ids = B.reshape(tokens, (1, rows))
+        else:
+            ids = TensorData((1, rows), "i32", np.asarray(tokens, np.int32))
+        key = (tuple(seqs), tuple(counts))
+        if self._batch[0] != key:
+            starts = np.concatenate([[0], np.cumsum(counts)])
+            self._batch = (key, TensorData((len(seqs), self.table.shape[1]), "i32", self.table[list(seqs)]), TensorData((len(seqs) + 1,), "i32", starts))
+        ends = TensorData((len(seqs),), "i32", lens)
+        self.pages = [Pages(k, v, *self._batch[1:], ends) for k, v in self.layers]
+        self.positions = TensorData((1, rows), "i32", np.concatenate([np.arange(n - c, n) for n, c in zip(lens, counts)]))
+        tape = Tape()
+        ctx = Ctx(tape, B, batch=self)
+        x = gptBlocks(ctx, cfg, self.params, ids)
+        logits = None
+        if len(wanted):
+            x = ag.reshape(ctx, x, [rows, cfg.nEmbd])
+            if list(wanted) != list(range(rows)):
+                last = (np.cumsum(counts) - 1)[list(wanted)]
+                x = ag.embedding(ctx, x, TensorData((len(wanted),), "i32", last))
+            x = ag.layerNorm(ctx, x, self.params["lnF"]["weight"], self.params["lnF"]["bias"], 1e-5)
+            logits = ag.matmulTransposed(ctx, x, self.params["lmHead"])
+        tape.clear(releaseTensor, logits)
+        if releaseTensor is not None:
+            for t in (ids, ends, self.positions):
+                releaseTensor(t)
+        self.lens[list(seqs)] = lens
+        return None if logits is None else logits.data
+
+    def attention(self, ctx: Ctx, qkv: Variable, nHead: int, scale: float, softCap: float) -> Variable:
+        """Of the next layer (gptBlocks asks for each in turn): the new tokens' keys and values go into its pages, their queries over them."""
+        pages = self.pages.pop(0)
+        self.backend.pagedAppend(pages, qkv.data, nHead)
+        r = self.backend.pagedAttention(pages, qkv.data, nHead, scale, softCap)
+        out = Variable(r["output"], False)
+        ctx.tape.record(out, [], None)
+        return out
+
+    def close(self):
+        for k, v in self.layers:
+            self.backend.releaseGpuTensor(k)
+            self.backend.releaseGpuTensor(v)
+        self.layers = []

@@ -146,7 +146,9 @@ def transformerBlock(ctx: Ctx, x: Variable, layer: dict, cfg: ModelConfig, Bt: i
         ctx.keptQkv.append(qkv)
     cap = cfg.softCap if cfg.softCap is not None else 30.0
     scl = 1 / math.sqrt(D)
-    if cfg.attention == "heads" and cfg.dropout == 0 and ag._has(Bk, "attentionQkv") and flashHeadSize(D):
+    if ctx.batch is not None:
+        concat = ctx.batch.attention(ctx, qkv, H, scl, cap)
+    elif cfg.attention == "heads" and cfg.dropout == 0 and ag._has(Bk, "attentionQkv") and flashHeadSize(D):
         concat = ag.causalSelfAttention(ctx, qkv, Bt, T, H, scl, cap)
     else:
         qF, kF, vF = ag.sliceQkv(ctx, qkv)
@@ -217,7 +219,7 @@ def gptBlocks(ctx: Ctx, cfg: ModelConfig, params: dict, tokens: TensorData, trai
     Bt, T = tokens.shape
     tok = ag.embedding(ctx, params["wte"], tokens)
     key = (id(backend), Bt, T)
-    pos = _pos_cache.get(key)
+    pos = _pos_cache.get(key) if ctx.batch is None else ctx.batch.positions
     if pos is None:
         pos = TensorData((Bt, T), "i32", np.tile(np.arange(T, dtype=np.int32), Bt))
         _pos_cache[key] = pos

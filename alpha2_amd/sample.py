@@ -1,18 +1,19 @@
 """Text generation from a trained model (packages/train/src/sample.ts:23-201): for each new token the logits behind the last
 blockSize tokens (by a forward pass over them, or from kept keys and values where the model allows it: decode.py), then greedy /
 top-k / nucleus / full-softmax selection on the host with the reference's arithmetic (f32 storage, double accumulation, stable
-descending sorts) and its use of the seeded rng (one draw per sampled token)."""
+descending sorts) and its use of the seeded rng (one draw per sampled token).  sampleTokensBatch does this for several prompts at
+once, one pass of the model for all, their keys and values in pages, the selection on the device."""
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Callable, Optional, Sequence
+from typing import Callable, List, Optional, Sequence
 
 import numpy as np
 
 from .autograd import Tape
 from .backend import TensorData
-from .decode import KeptContext, mayMove
+from .decode import KeptContext, PagedContext, mayMove
 from .model import ModelConfig, gptForward
 
 
@@ -130,6 +131,88 @@ def sampleTokens(config: ModelConfig, params: dict, backend, rng, promptTokens: 
         if kept is not None:
             kept.close()
     return tokens[:currentLen]
+
+
+def sampleTokensBatch(config: ModelConfig, params: dict, backend, rngs: Sequence, prompts: Sequence[Sequence[int]], sampleConfigs,
+                      releaseTensor: Optional[Callable] = None, flushGpu: Optional[Callable] = None) -> List[np.ndarray]:
+    """What sampleTokens returns for each prompt with its own rng (and, from a sequence of SampleConfig, its own options): a sequence's
+    tokens do not depend on which others are run with it, but for sums taken in other orders.  One forward pass serves a token of every
+    sequence; where model or backend do not allow that, the sequences are run one after the other."""
+    prompts = [np.asarray(p, dtype=np.int32).reshape(-1) for p in prompts]
+    configs = [sampleConfigs] * len(prompts) if isinstance(sampleConfigs, SampleConfig) else list(sampleConfigs)
+    if len(rngs) != len(prompts) or len(configs) != len(prompts):
+        raise ValueError(f"{len(prompts)} prompts, {len(rngs)} rngs, {len(configs)} options")
+    for p in prompts:
+        if not 0 < p.size <= config.blockSize:
+            raise ValueError(f"prompt of {p.size} tokens, where 1 to blockSize {config.blockSize} are taken")
+        if p.min() < 0 or p.max() >= config.vocabSize:
+            raise ValueError(f"prompt with tokens outside 0 .. {config.vocabSize - 1}")
+    wanted = [min(p.size + max(c.steps, 0), config.blockSize) for p, c in zip(prompts, configs)]
+    run = [i for i in range(len(prompts)) if wanted[i] > prompts[i].size]
+    kept = PagedContext.of(config, params, backend, [wanted[i] for i in run]) if run else None
+    if kept is None:
+        return [sampleTokens(config, params, backend, r, p, c, releaseTensor, flushGpu) for r, p, c in zip(rngs, prompts, configs)]
+    tokens = [np.concatenate([p, np.zeros(n - p.size, np.int32)]) for p, n in zip(prompts, wanted)]
+    at = [int(p.size) for p in prompts]                                     # tokens known on the host
+    topp = [min(1.0, max(0.0, c.topp)) if c.topp is not None and math.isfinite(c.topp) else 1.0 for c in configs]
+    options, chosen = {}, []
+
+    def choose(logits: TensorData, seqs: tuple) -> TensorData:
+        if seqs not in options:
+            options.clear()
+            options[seqs] = [TensorData((len(seqs),), dtype, np.array(list(values))) for dtype, values in (
+                ("f32", (configs[i].temperature for i in seqs)), ("i32", (configs[i].topk for i in seqs)), ("f32", (topp[i] for i in seqs)))]
+        # (a draw that f32 would round to 1 stays below it)
+        draws = np.array([rngs[i].next() if configs[i].temperature > 0 else 0.0 for i in seqs]).astype(np.float32)
+        r = backend.sampleRows(logits, TensorData((len(seqs),), "f32", np.minimum(draws, np.float32(1 - 2.0 ** -24))), *options[seqs])
+        if releaseTensor is not None:
+            releaseTensor(logits)
+        chosen.append((seqs, r["tokens"]))
+        return r["tokens"]
+
+    def settle():
+        for seqs, t in chosen:
+            for i, token in zip(seqs, t.data):
+                tokens[i][at[i]] = token
+                at[i] += 1
+        chosen.clear()
+
+    try:
+        # the prompts, as many rows at a time as the memory for activations is meant for: a long one over several passes
+        done = [0] * len(run)
+        while any(done[j] < prompts[i].size for j, i in enumerate(run)):
+            room, part = kept.MOST_ROWS, []
+            for j, i in enumerate(run):
+                n = min(room, int(prompts[i].size) - done[j])
+                if n > 0:
+                    part.append((j, prompts[i][done[j]:done[j] + n]))
+                    room -= n
+            for j, new in part:
+                done[j] += new.size
+            ready = [k for k, (j, _) in enumerate(part) if done[j] == prompts[run[j]].size]
+            logits = kept.forward([j for j, _ in part], [new.size for _, new in part], np.concatenate([new for _, new in part]), ready, releaseTensor)
+            if ready:
+                choose(logits, tuple(run[part[k][0]] for k in ready))
+        step, last, made = 1, None, [1] * len(run)
+        while True:
+            live = [j for j, i in enumerate(run) if made[j] < wanted[i] - prompts[i].size]
+            if not live:
+                break
+            seqs = tuple(run[j] for j in live)
+            if last is None or last[0] != seqs:                             # (the sequences that are left stay in order)
+                settle()
+                last = (seqs, np.array([tokens[i][at[i] - 1] for i in seqs], np.int32))
+            logits = kept.forward(live, [1] * len(live), last[1], range(len(live)), releaseTensor)
+            last = (seqs, choose(logits, seqs))
+            for j in live:
+                made[j] += 1
+            if flushGpu is not None and (step & 7) == 7:
+                flushGpu()
+            step += 1
+        settle()
+    finally:
+        kept.close()
+    return tokens
 
 
 def sample(config: ModelConfig, params: dict, backend, rng, encode: Callable, decode: Callable, prompt: str, sampleConfig: SampleConfig,

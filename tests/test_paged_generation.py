@@ -1,0 +1,117 @@
+"""What generation from several prompts refuses, and what runs where nothing is kept in pages, without a GPU."""
+import numpy as np
+import pytest
+
+from alpha2_amd import FastHipBackend, HipBackend, Pages, TensorData
+from alpha2_amd import sample
+from alpha2_amd.decode import PagedContext
+from alpha2_amd.model import ModelConfig
+from alpha2_amd.sample import SampleConfig, sampleTokensBatch
+
+
+def T(*shape, dtype="f32", store=None):
+    t = TensorData(shape, dtype, np.zeros(shape))
+    t.store = store or dtype
+    return t
+
+
+def I(*shape):
+    return T(*shape, dtype="i32")
+
+
+def pages(store="f32", **other):
+    parts = dict(k=T(4, 16, 2, 8, store=store), v=T(4, 16, 2, 8, store=store), table=I(3, 5), starts=I(4), lens=I(3))
+    return Pages(**{**parts, **other})
+
+
+@pytest.fixture(params=[HipBackend, FastHipBackend])
+def backend(request):
+    return request.param.__new__(request.param)         # what is refused here is so before the library is called
+
+
+@pytest.mark.parametrize("other", [dict(k=T(4, 16, 16)), dict(v=T(4, 16, 2, 16)), dict(v=T(4, 16, 2, 8, store="bf16")), dict(table=I(15)),
+                                   dict(table=I(2, 5)), dict(starts=I(3)), dict(lens=I(4))])
+def test_pages_that_do_not_fit(other):
+    with pytest.raises(ValueError):
+        pages(**other)
+
+
+@pytest.mark.parametrize("name", ["table", "starts", "lens"])
+def test_indices_of_another_type(name):
+    with pytest.raises(TypeError):
+        pages(**{name: T(*getattr(pages(), name).shape)})
+
+
+@pytest.mark.parametrize("shape,heads,rotary", [((5, 64), 3, None), ((5, 48), 0, None), ((80,), 6, None), ((5, 80), 6, (32,)), ((5, 32), -2, None)])
+def test_projections_that_do_not_fit(backend, shape, heads, rotary):
+    with pytest.raises(ValueError):
+        backend.pagedAppend(pages(), T(*shape), heads, rotary and T(*rotary))
+
+
+@pytest.mark.parametrize("shape,heads", [((5, 40), 6), ((5, 48), 0), ((48,), 6)])
+def test_queries_that_do_not_fit(backend, shape, heads):
+    with pytest.raises(ValueError):
+        backend.pagedAttention(pages(), T(*shape), heads, 1.0)
+
+
+def test_tensors_of_another_type(backend):
+    with pytest.raises(TypeError):
+        backend.pagedAppend(pages(), I(5, 80), 6)
+    with pytest.raises(TypeError):
+        backend.pagedAttention(pages(), I(5, 48), 6, 1.0)
+    with pytest.raises(TypeError):
+        backend.sampleRows(I(5, 48), T(5))
+    if type(backend) is HipBackend:                      # (the fast one makes a copy of the pages' type)
+        with pytest.raises(TypeError):
+            backend.pagedAppend(pages("bf16"), T(5, 80), 6)
+        with pytest.raises(TypeError):
+            backend.pagedAttention(pages(), T(5, 48, store="bf16"), 6, 1.0)
+
+
+@pytest.mark.parametrize("name,t,error", [("uniform", T(4), ValueError), ("uniform", I(5), TypeError), ("temperature", T(5, 1), ValueError),
+                                          ("temperature", T(5, store="bf16"), TypeError), ("topk", T(5), TypeError), ("topk", I(6), ValueError),
+                                          ("topp", I(5), TypeError), ("minp", T(1), ValueError)])
+def test_options_that_do_not_fit(backend, name, t, error):
+    with pytest.raises(error):
+        backend.sampleRows(T(5, 48), **{"uniform": T(5), name: t})
+    with pytest.raises(ValueError):
+        backend.sampleRows(T(48), T(48))
+
+
+CFG = dict(vocabSize=20, blockSize=12, nLayer=1, nEmbd=16, nHead=2)
+
+
+@pytest.mark.parametrize("prompts,rngs,configs", [([[]], 1, SampleConfig()), ([[1] * 13], 1, SampleConfig()), ([[1, 20]], 1, SampleConfig()), ([[-1]], 1, SampleConfig()),
+                                                  ([[1], [2]], 1, SampleConfig()), ([[1], [2]], 2, [SampleConfig()])])
+def test_prompts_that_are_refused(prompts, rngs, configs):
+    with pytest.raises(ValueError):
+        sampleTokensBatch(ModelConfig(**CFG), {}, None, [None] * rngs, prompts, configs)
+
+
+@pytest.mark.parametrize("more", [dict(attention="unfused"), dict(attention="reference-flash"), dict(dropout=0.1), dict(nEmbd=24, nHead=2), dict(nEmbd=15), dict(nEmbd=512, nHead=2)])
+def test_models_whose_sequences_are_run_one_by_one(monkeypatch, more):
+    cfg, calls = ModelConfig(**{**CFG, **more}), []
+    assert PagedContext.of(cfg, {}, HipBackend.__new__(HipBackend), [3]) is None
+    assert PagedContext.of(ModelConfig(**CFG), {}, object(), [3]) is None
+    monkeypatch.setattr(sample, "sampleTokens", lambda *a: calls.append(a) or np.array(a[4]))
+    configs = [SampleConfig(steps=3), SampleConfig(steps=4)]
+    got = sampleTokensBatch(cfg, "params", object(), ["a", "b"], [[1], [2, 3]], configs, "release", "flush")
+    assert [g.tolist() for g in got] == [[1], [2, 3]]
+    assert [(a[3], a[5], a[6], a[7]) for a in calls] == [("a", configs[0], "release", "flush"), ("b", configs[1], "release", "flush")]
+
+
+def test_more_tokens_than_a_sequence_was_given_room_for():
+    kept = PagedContext(ModelConfig(**CFG), {}, None, [3, 12])
+    kept.lens[:] = 2, 12
+    for seqs, counts in (([0], [2]), ([1], [1]), ([0, 0], [1, 1]), ([0], [0])):
+        with pytest.raises(ValueError):
+            kept.forward(seqs, counts, np.zeros(sum(counts), np.int32), [], None)
+
+
+def test_every_sequence_has_pages_of_its_own():
+    kept = PagedContext(ModelConfig(**{**CFG, "blockSize": 300}), {}, None, [1, 64, 65, 300, 128])
+    need = [1, 1, 2, 5, 2]
+    owned = [set(kept.table[i, :n].tolist()) for i, n in enumerate(need)]
+    assert sorted(p for s in owned for p in s) == list(range(sum(need)))
+    for i, s in enumerate(owned):
+        assert set(kept.table[i].tolist()) == s
