@@ -286,6 +286,21 @@ struct Bins {
   }
 };
 static_assert(BINS == 1 << 11, "the shift of a bin's bins");
+// Is there only one bf16 number among those between lo and hi that fall into bin b?  Rows of bf16 have thousands of equal logits.
+__device__ __forceinline__ bool one_of_bin(const Bins &bin, int b, float lo, float hi, float &only) {
+  const uint32_t first = order_of(hi) >> 16, last = order_of(lo) >> 16;
+  if (first - last > 6) return false;
+  int different = 0;
+  only = 0.f;
+#pragma unroll 1
+  for (uint32_t o = first; o + 1 > last; o--) {
+    const float x = __uint_as_float((o & 0x8000u ? o ^ 0x8000u : o ^ 0xffffu) << 16) + 0.f;
+    const bool in = x >= lo && x <= hi && bin(x) == b && !(different && x == only);
+    only = in ? x : only;
+    different += in;
+  }
+  return different == 1;
+}
 
 // s.bins[level] to running sums; the sum of all
 template <int THREADS>
@@ -524,10 +539,12 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
         const int b = same(s.found);
         base = same(s.found_before);
         int which = 0, n = 0;
-        const bool listed = !level && goal == TOKEN && (b == have[0] || b == have[1]);
-        float lo, hi;
+        float lo, hi, value = 0.f;
         bin.around(b, least, lo, hi);
-        if (listed) {
+        bool equal = N == 8 && one_of_bin(bin, b, lo, hi, value);
+        const bool listed = !equal && !level && goal == TOKEN && (b == have[0] || b == have[1]);
+        if (equal) {
+        } else if (listed) {
           which = b == have[0] ? 0 : 1;
           n = members[which];
         } else {
@@ -539,6 +556,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
             find_bin<THREADS>(s, 0, 0, then);
             too = same(s.found);
             if (too != b) bin.around(too, least, lo2, hi2);
+            if (N == 8 && too != b && one_of_bin(bin, too, lo2, hi2, value)) { too = b; lo2 = INFINITY; hi2 = -INFINITY; }
           } else if (!level && goal == TOKEN) {  // (neither list: the first is made anew)
             __syncthreads();
             if (t == 0) s.listed[0] = 0;
@@ -557,7 +575,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
             members[1] = same(s.listed[1]);
           } else if (goal == END) have[0] = -1;
         }
-        if (n <= LIST) {
+        if (!equal && n <= LIST) {
           if (!(listed && which == 0)) sort_list<THREADS>(s, s.list[which], n);      // (the nucleus's is sorted)
           uint64_t w[EACH], sum = 0, dummy;
 #pragma unroll
@@ -584,23 +602,27 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
           f = Found{entry_logit(e), entry_index(e), same(s.found_before), 0};
           break;
         }
-        const float from = lo, to = hi;
-        lo = INFINITY;
-        hi = -INFINITY;
-        row.hits(from, to, INFINITY, -INFINITY, [&](float l, int) {
-          const bool in = bin(l) == b;
-          lo = in ? fminf(lo, l) : lo;
-          hi = in ? fmaxf(hi, l) : hi;
-        });
-        block_bounds<THREADS>(lo, hi, s);
-        if (lo == hi) {                          // equal ones: how many of them it takes
-          const uint64_t w = same(weight(lo));
-          uint32_t few = 1, many = (uint32_t)n;
+        if (!equal) {
+          const float from = lo, to = hi;
+          lo = INFINITY;
+          hi = -INFINITY;
+          row.hits(from, to, INFINITY, -INFINITY, [&](float l, int) {
+            const bool in = bin(l) == b;
+            lo = in ? fminf(lo, l) : lo;
+            hi = in ? fmaxf(hi, l) : hi;
+          });
+          block_bounds<THREADS>(lo, hi, s);
+          equal = lo == hi;
+          value = lo;
+        }
+        if (equal) {                             // how many of them it takes
+          const uint64_t w = same(weight(value));
+          uint32_t few = 1, many = (uint32_t)row.V;
           for (int i = 0; i < 20 && few < many; i++) {
             const uint32_t middle = few + (many - few) / 2;
             if (base + middle * w >= mark) many = middle; else few = middle + 1;
           }
-          f = Found{lo, -1, base + few * w, base};
+          f = Found{value, -1, base + few * w, base};
           break;
         }
         least = lo;
