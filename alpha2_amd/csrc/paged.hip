@@ -183,7 +183,7 @@ int32_t append(AppendArgs &a, bool neighbours) {
                                      : (int64_t)(a.heads + a.kv_heads) * a.of_turned.divisor + (int64_t)a.kv_heads * pieces;
   if (items > INT32_MAX / MOST_ROWS) return fail(AH_ERR_UNSUPPORTED, "ah_paged_append: %lld pieces to a row", (long long)items);
   a.of_row = quotient_by((uint32_t)items);
-  const int64_t want = cdiv(2048, items), fill = cdiv(a.c.rows, (int64_t)4 * num_cus());
+  const int64_t want = cdiv(1024, items), fill = cdiv(a.c.rows, (int64_t)4 * num_cus());
   a.group = (int32_t)(want < fill ? want : fill);
   if (a.group > MOST_ROWS) a.group = MOST_ROWS;
   const dim3 grid((unsigned)cdiv(a.c.rows, a.group));
