@@ -62,7 +62,7 @@ template <int TILE>
 __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan, int group, int index, bool by_tile) {
   const int lane = threadIdx.x & 63;
   auto sequence = [&](int s) { return s < c.seqs ? sequence_of(c.starts[s], c.starts[s + 1], c.lens[s], c.rows) : Sequence{0, 0, 0}; };
-  Unit u;
+  Unit u{};
   u.seq = -1;
   u.span = INT32_MAX;
   Sequence mine = sequence(lane);
@@ -107,6 +107,10 @@ __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan,
     }
     base += __shfl(upto, 63);
   }
+  // all lanes hold the same: scalars from here on
+  auto scalar = [](int &v) { v = __builtin_amdgcn_readfirstlane(v); };
+  scalar(u.s.first); scalar(u.s.count); scalar(u.s.len);
+  scalar(u.seq); scalar(u.tile); scalar(u.part); scalar(u.parts); scalar(u.span); scalar(u.own); scalar(u.first);
   return u;
 }
 
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
   constexpr int KS = D / 32, DB = D / 16, NV = D / 16, TILE = 16;
   __shared__ __attribute__((aligned(16))) char own[4 * G::WAVE_BYTES];
   __shared__ float tops[4][TILE], sums[4][TILE];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % a.kv_heads;
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
@@ -449,7 +453,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = G::LOADS;
   constexpr bool CAPPED = MODE == 1;
   __shared__ __attribute__((aligned(1024))) char Ks[2][G::BYTES], Vs[2][G::BYTES];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
+  __shared__ int specials;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
   const int head = blockIdx.x % a.kv_heads;
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
@@ -481,7 +486,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; e++) o[d][e] = 0.f;
   float m = CAPPED ? c2 : -INFINITY, l = 0.f;
-  bool specials = false;
+  if (threadIdx.x == 0) specials = 0;
+  const int all_see = u.limit(u.tile * TILE, a.group);                        // every column of the workgroup sees the positions before this one
 
   // What this lane fetches: piece `lane % PIECES`, as it lands, of row base + its_row(n).  Positions past the end look at the last one's entry, so that nothing
   // here branches: page and row in 16-byte pieces, one multiplication each, and the row of zeros or NaN where they name no place.
@@ -536,6 +542,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
       entries(base + 2 * ST);
     }
     const char *kt = Ks[cur], *vt = Vs[cur];
+    if (base + ST > all_see && all_see < end) {
+      bool some = false;
+#pragma unroll
+      for (int e = 0; e < G::BYTES; e += 256 * 16) {
+        bf16x8 *at = reinterpret_cast<bf16x8 *>(Vs[cur] + e + threadIdx.x * 16);
+        const bool special = has_special(*at);
+        if (special) *at = finite_of(*at);
+        some |= special;
+      }
+      if (some) specials = 1;
+      __syncthreads();
+    }
 #pragma unroll 1
     for (int sub = 0; sub < ST; sub += 32) {
       const int kv0 = base + sub;
@@ -584,34 +602,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
         for (int e = 0; e < 16; e++) { s[e] = exp2_fast(fmaf(s[e], slope, shift)); l += s[e]; }
       }
       const bf16x8 p0 = acc_to_b(s, 0), p1 = acc_to_b(s, 1);
-      bool special = false;
-      if (edge && least < end) {                                   // some columns see less than others
-        keep_branch();
-        const char *again = apart(vt);
-#pragma unroll 1
-        for (int d = 0; d < DB; d++) special |= has_special(values(again, sub, 0, d)) | has_special(values(again, sub, 1, d));
-        special = __any(special);
-      }
-      if (!special) {
 #pragma unroll
-        for (int d = 0; d < DB; d++) {
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 0, d), p0, o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 1, d), p1, o[d], 0, 0, 0);
-        }
-      } else {
-        specials = true;
-        const char *again = apart(vt);
-#pragma unroll
-        for (int d = 0; d < DB; d++) {
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_of(values(again, sub, 0, d)), p0, o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(finite_of(values(again, sub, 1, d)), p1, o[d], 0, 0, 0);
-        }
+      for (int d = 0; d < DB; d++) {
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 0, d), p0, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 1, d), p1, o[d], 0, 0, 0);
       }
     }
   }
+  __syncthreads();
   if (specials) {
     keep_branch();
-    for (int kv = least > begin ? begin + (least - begin) / 32 * 32 : begin; kv < wave_end; kv++) {
+    for (int kv = all_see > begin ? begin + (all_see - begin) / ST * ST : begin; kv < wave_end; kv++) {
       const int64_t at = position_place(a.c, u.seq, kv);
       if (at < 0) continue;
 #pragma unroll
@@ -664,7 +665,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
   __shared__ __attribute__((aligned(16))) float joined[4 * TILE * O_PITCH];
   __shared__ float tops[4][TILE], sums[4][TILE];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % a.kv_heads;
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, blockIdx.x / a.kv_heads, false);
   if (u.seq < 0 || (u.part > 0 && u.part >= u.parts)) return;
