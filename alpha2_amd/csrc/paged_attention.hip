@@ -432,6 +432,11 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 // one barrier to a tile.  The tiles come by global_load_lds, 16 bytes to a lane from wherever its position's page lies, past the registers; what does not
 // exist is fetched from rows of zeros or NaN.  A wave's 1 KB lands in lane order, so rows cannot be padded: the 16-byte pieces of a row are permuted instead
 // (by the lane that fetches them), so that 16 rows' same piece and four rows' same 64 bytes each meet all 64 banks.
+// The two tiles are arrays of their own, and the loop is written out for both: an LDS read that may touch what a load under way writes waits for it, and
+// the compiler keeps them apart by the array.  Both halves of a tile's scores are taken together, so that the values (whose reads wait all the same) come
+// late.  Two sequences, chunks of 2048 and 1200 behind 14336 and 5058 positions, 32 heads of 128 on 8: 746 us, 840 TFLOP/s of the 1218 that a large product
+// reaches; one array and a half at a time, 791; the values' finite form chosen in the loop and not in LDS, 989.  Bound by the vector
+// instructions of the softmax and by waiting between them and the matrix ones, two waves to a SIMD.
 // MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself for the maximum (attention_bf16.hip); 2: a larger cap.
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
@@ -452,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   using G = RowsTile<D>;
   constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = G::LOADS;
   constexpr bool CAPPED = MODE == 1;
-  __shared__ __attribute__((aligned(1024))) char Ks[2][G::BYTES], Vs[2][G::BYTES];
+  __shared__ __attribute__((aligned(1024))) char Ks0[G::BYTES], Vs0[G::BYTES], Ks1[G::BYTES], Vs1[G::BYTES];
   __shared__ int specials;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
   const int head = blockIdx.x % a.kv_heads;
@@ -502,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
     }
   };
   const uint32_t pages = (uint32_t)a.c.pages;
-  auto load = [&](int buf, int base) {
+  auto load = [&](char *kt, char *vt, int base) {
 #pragma unroll
     for (int n = 0; n < N; n++) {
       const int r = its_row(n);
@@ -512,8 +517,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
       const uint16_t *k = (const uint16_t *)nothing[0], *v = k;
       k = wanted ? there ? K + at * 8 : (const uint16_t *)nothing[1] : k;
       v = wanted && there ? V + at * 8 : v;
-      __builtin_amdgcn_global_load_lds((glb_void *)k, (lds_void *)(Ks[buf] + (wave * N + n) * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_void *)v, (lds_void *)(Vs[buf] + (wave * N + n) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void *)k, (lds_void *)(kt + (wave * N + n) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void *)v, (lds_void *)(vt + (wave * N + n) * 1024), 16, 0, 0);
     }
   };
   const int k_turned = G::turned(lr);
@@ -530,23 +535,21 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   };
   if (begin < end) {
     entries(begin);
-    load(0, begin);
+    load(Ks0, Vs0, begin);
     entries(begin + ST);
   }
-  int cur = 0;
-  for (int base = begin; base < end; base += ST, cur ^= 1) {
+  auto step = [&](char *kt, char *vt, char *next_kt, char *next_vt, int base) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // this tile is there, for all behind the barrier
     __syncthreads();
     if (base + ST < end) {
-      load(cur ^ 1, base + ST);
+      load(next_kt, next_vt, base + ST);
       entries(base + 2 * ST);
     }
-    const char *kt = Ks[cur], *vt = Vs[cur];
     if (base + ST > all_see && all_see < end) {
       bool some = false;
 #pragma unroll
       for (int e = 0; e < G::BYTES; e += 256 * 16) {
-        bf16x8 *at = reinterpret_cast<bf16x8 *>(Vs[cur] + e + threadIdx.x * 16);
+        bf16x8 *at = reinterpret_cast<bf16x8 *>(vt + e + threadIdx.x * 16);
         const bool special = has_special(*at);
         if (special) *at = finite_of(*at);
         some |= special;
@@ -554,60 +557,78 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
       if (some) specials = 1;
       __syncthreads();
     }
-#pragma unroll 1
-    for (int sub = 0; sub < ST; sub += 32) {
-      const int kv0 = base + sub;
-      if (kv0 >= wave_end) break;                                  // (the same for the wave) nothing for its columns
-      f32x16 s;
+    if (base >= wave_end) return;                                  // (the same for the wave) nothing for its columns
+    f32x16 s[2];
 #pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = 0.f;
+    for (int b = 0; b < 2; b++) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(kt, sub, ks), qf[ks], s, 0, 0, 0);
-      const bool edge = kv0 + 32 > min(least, end);
-      if (MODE == 1) {
+      for (int e = 0; e < 16; e++) s[b][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = exp2_fast(rcp_fast(fmaf(exp2_fast(s[e] * c1), ic2, ic2)));
-        if (edge) {
-          keep_branch();
+      for (int ks = 0; ks < KS; ks++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(kt, 32 * b, ks), qf[ks], s[b], 0, 0, 0);
+    }
+    const bool edge = base + ST > min(least, end);
+    if (MODE == 1) {
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[e] : 0.f;
-        }
+      for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) l += s[e];
-      } else {
-        if (MODE == 2) {
+        for (int e = 0; e < 16; e++) s[b][e] = exp2_fast(rcp_fast(fmaf(exp2_fast(s[b][e] * c1), ic2, ic2)));
+      if (edge) {
+        keep_branch();
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[e] * c1) + 1.0f), c2);
-        }
-        if (edge) {
-          keep_branch();
+        for (int b = 0; b < 2; b++)
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[e] = kv0 + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[e] : -INFINITY;
-        }
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-        top = max_lane<32>(top);
-        if (__any(top > m)) {
-          const float larger = fmaxf(m, top), keep = exp2_fast((m - (larger == -INFINITY ? 0.f : larger)) * slope);
-          l *= keep;
-#pragma unroll
-          for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] *= keep;
-          m = larger;
-        }
-        const float shift = (m == -INFINITY ? 0.f : -m) * slope;
-#pragma unroll
-        for (int e = 0; e < 16; e++) { s[e] = exp2_fast(fmaf(s[e], slope, shift)); l += s[e]; }
+          for (int e = 0; e < 16; e++) s[b][e] = base + 32 * b + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[b][e] : 0.f;
       }
-      const bf16x8 p0 = acc_to_b(s, 0), p1 = acc_to_b(s, 1);
+    } else {
+      if (MODE == 2) {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[b][e] = fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[b][e] * c1) + 1.0f), c2);
+      }
+      if (edge) {
+        keep_branch();
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[b][e] = base + 32 * b + 8 * (e >> 2) + 4 * lk + (e & 3) < limit ? s[b][e] : -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = fmaxf(top, s[b][e]);
+      top = max_lane<32>(top);
+      if (__any(top > m)) {
+        const float larger = fmaxf(m, top), keep = exp2_fast((m - (larger == -INFINITY ? 0.f : larger)) * slope);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[d][e] *= keep;
+        m = larger;
+      }
+      const float shift = (m == -INFINITY ? 0.f : -m) * slope;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[b][e] = exp2_fast(fmaf(s[b][e], slope, shift));
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const bf16x8 p0 = acc_to_b(s[b], 0), p1 = acc_to_b(s[b], 1);
+#pragma unroll
+      for (int e = 0; e < 16; e++) l += s[b][e];
 #pragma unroll
       for (int d = 0; d < DB; d++) {
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 0, d), p0, o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, sub, 1, d), p1, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, 32 * b, 0, d), p0, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(vt, 32 * b, 1, d), p1, o[d], 0, 0, 0);
       }
     }
+  };
+  for (int base = begin; base < end; base += 2 * ST) {
+    step(Ks0, Vs0, Ks1, Vs1, base);
+    if (base + ST < end) step(Ks1, Vs1, Ks0, Vs0, base + ST);
   }
   __syncthreads();
   if (specials) {
@@ -657,9 +678,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // each piece of a page is read once by a workgroup.  With 32 columns to a wave, each streaming all positions, a batch of prompts of 12 heads of 64
 // took 254 us; with the positions cut, 168, and with one block as long, but chunks of 512 in 4096 positions, 16 heads of 64: 398 us, two 369 (88 TFLOP/s of
 // the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.
-// a score through the cap: cap tanh(x), x = score / cap
-__device__ __forceinline__ float capped_f32(float x, float cap) { return cap * (fabsf(x) < TANH_SMALL ? tanh_small(x) : tanh_large(x)); }
-
 template <int D, int NC>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
@@ -784,8 +802,15 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a
 #pragma unroll
       for (int r = 0; r < 4; r++) s[r] *= factor;
       if (a.cap > 0.f) {
+        const f32x4 x = s;
+        const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
-        for (int r = 0; r < 4; r++) s[r] = capped_f32(s[r], a.cap);
+        for (int r = 0; r < 4; r++) s[r] = a.cap * tanh_small(x[r]);
+        if (__any(!(most < TANH_SMALL))) {            // (scores are seldom near the cap)
+          keep_branch();
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[r] = fabsf(x[r]) < TANH_SMALL ? s[r] : a.cap * tanh_large(x[r]);
+        }
       }
       if (edge) {
         keep_branch();
