@@ -178,19 +178,22 @@ template <> __device__ __forceinline__ void store4<uint16_t>(uint16_t *p, float 
 }
 constexpr float LN2 = 0.693147180559945309f;
 
-constexpr int join_slices(int tile, int d) { return tile * d / 4 > 256 ? tile * d / 4 / 256 : 1; }
-// Joins the parts of a tile: a thread to four features of a column, a workgroup to 256 such of a tile and kv head (a workgroup to all 128 columns of a
-// tile has too few of them at work: at 4 sequences of 8 kv heads in 16 parts, 32 columns each, 63 us against 39).  Maxima are logarithms to base 2.
+// Joins the parts of a tile: a thread to four features of a column.  Few columns can have many parts: there four waves share them, each its own sum with its
+// own running maximum, and are joined in LDS; a workgroup has 64 such fours.  A tile of rows has many columns, and a workgroup 256 fours of it.
+constexpr int join_ways(int tile) { return tile <= 32 ? 4 : 1; }
+constexpr int join_slices(int tile, int d) { return tile * d / 4 * join_ways(tile) / 256; }
 template <class T, int TILE, int D>
 __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
-  constexpr int SLICES = join_slices(TILE, D);
-  const int index = blockIdx.x / SLICES, head = index % a.kv_heads;
+  constexpr int SLICES = join_slices(TILE, D), WAYS = join_ways(TILE), ITEMS = 256 / WAYS;
+  __shared__ float4 products[WAYS][ITEMS];
+  __shared__ float tops[WAYS][ITEMS], sums[WAYS][ITEMS];
+  const int index = blockIdx.x / SLICES, head = index % a.kv_heads, slice = blockIdx.x % SLICES;
   // the units of the tiles before this one have to be known: find_unit by tile gives those of the sequence, the others are added up here
   const Unit u = find_unit<TILE>(a.c, a.plan, a.group, index / a.kv_heads, true);
   if (u.seq < 0 || u.parts == 1) return;
-  const int e = blockIdx.x % SLICES * 256 + threadIdx.x, col = e / (D / 4), f = e % (D / 4) * 4, i = u.tile * TILE + col;
   const int columns = u.s.count * a.group;
-  if (u.tile * TILE + (int)(blockIdx.x % SLICES) * 256 / (D / 4) >= columns) return;          // (all of it)
+  if (u.tile * TILE + slice * ITEMS / (D / 4) >= columns) return;          // (all of the workgroup)
+  const int way = threadIdx.x / ITEMS, item = threadIdx.x % ITEMS, e = slice * ITEMS + item, col = e / (D / 4), f = e % (D / 4) * 4, i = u.tile * TILE + col;
   int before = 0;
   for (int s0 = 0; s0 < u.seq; s0 += 64) {
     const int s = s0 + (threadIdx.x & 63);
@@ -202,22 +205,30 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
   const int64_t first = before + u.first;
-  if (i >= columns || col >= TILE || f >= a.head_dim) return;
+  const bool some = i < columns && f < a.head_dim;
   const int64_t pitch = (int64_t)a.kv_heads * (TILE * (D + 2));
   const float *part = part_at<TILE, D>(a.plan, first * a.kv_heads + head), *stats = part + TILE * D + col;
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int p = 0; p < u.parts; p++) m = fmaxf(m, stats[p * pitch]);
-  const float shift = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](float more_m, float more_l, const float4 &x) {
+    const float top = fmaxf(m, more_m), shift = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - shift), w = exp2_fast(more_m - shift);
+    l = fmaf(more_l, w, l * keep);
+    o.x = fmaf(x.x, w, o.x * keep); o.y = fmaf(x.y, w, o.y * keep); o.z = fmaf(x.z, w, o.z * keep); o.w = fmaf(x.w, w, o.w * keep);
+    m = top;
+  };
+  if (some)
 #pragma unroll 4
-  for (int p = 0; p < u.parts; p++) {
-    const float w = exp2_fast(stats[p * pitch] - shift);
-    const float4 x = *reinterpret_cast<const float4 *>(part + p * pitch + col * D + f);
-    l = fmaf(stats[p * pitch + TILE], w, l);
-    o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    for (int p = way; p < u.parts; p += WAYS) join(stats[p * pitch], stats[p * pitch + TILE], *reinterpret_cast<const float4 *>(part + p * pitch + col * D + f));
+  if constexpr (WAYS > 1) {
+    products[way][item] = o;
+    tops[way][item] = m;
+    sums[way][item] = l;
+    __syncthreads();
+    if (way) return;
+#pragma unroll
+    for (int w = 1; w < WAYS; w++) join(tops[w][item], sums[w][item], products[w][item]);
   }
+  if (!some) return;
   l = column_sum(l, u.limit(i, a.group), a.c.capacity);
   const int64_t row = u.s.first + i / a.group, h = (int64_t)head * a.group + i % a.group;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
