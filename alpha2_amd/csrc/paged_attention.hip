@@ -926,7 +926,8 @@ constexpr int64_t PART_BYTES = int64_t(60) << 20;
 // cannot name more positions than a part has.  Otherwise about `wanted` units are cut: more of them even out ragged sequences, fewer are fewer to join.
 template <class T, int TILE, int D, class Kernel>
 int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
-  const int64_t tiles = cdiv((int64_t)a.c.rows * a.group, TILE) + a.c.seqs;                  // of one kv head, at most
+  // of one kv head, at most: every sequence with new tokens may end inside a tile
+  const int64_t ends = a.c.seqs < a.c.rows ? a.c.seqs : a.c.rows, tiles = ((int64_t)a.c.rows * a.group + ends * (TILE - 1)) / TILE;
   const int64_t slot = (int64_t)TILE * (D + 2) * sizeof(float) * a.kv_heads;
   const int64_t cus = num_cus();
   int64_t target = 0;
@@ -941,7 +942,9 @@ int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
     a.plan.parts = (float *)scratch((size_t)((tiles + target) * slot));
     if (!a.plan.parts) return fail(AH_ERR_OOM, "ah_paged_attention: no scratch for the parts of long sequences");
   }
-  const int64_t grid = (tiles + target) * a.kv_heads;
+  // parts are as many as positions over the launch's own length of a part, which is at least work / target, and at least `least`; and the rest of each
+  const int64_t parts = cdiv(a.c.capacity, least), units = target == 0 ? tiles : tiles * parts < tiles + target ? tiles * parts : tiles + target;
+  const int64_t grid = units * a.kv_heads;
   if (grid > INT32_MAX) return fail(AH_ERR_UNSUPPORTED, "ah_paged_attention: %lld workgroups", (long long)grid);
   launch_kernel(kernel, dim3((unsigned)grid), dim3(256), 0, a);
   AH_LAUNCH_CHECK();
