@@ -29,6 +29,7 @@ namespace {
 struct Plan {
   int32_t target;             // units that the positions of all tiles are cut into, about; 0: no cutting
   int32_t least;              // positions of a part, at least
+  int32_t whole;              // a sequence of as many is not cut
   float  *parts;              // what the units of tiles with more than one part leave: see part_at
 };
 struct AttendArgs {
@@ -56,6 +57,10 @@ template <int TILE>
 __device__ __forceinline__ int tiles_of(const Sequence &s, int group) { return (int)(((int64_t)s.count * group + TILE - 1) / TILE); }
 
 __device__ __forceinline__ int parts_of(int positions, int span) { return positions <= span ? 1 : (positions - 1) / span + 1; }
+__device__ __forceinline__ int parts_of(const Sequence &s, const PagedCache &c, const Plan &plan, int span) {
+  const int reach = min(s.len, c.capacity);
+  return reach <= plan.whole ? 1 : parts_of(reach, span);
+}
 
 // Unit `index` of the launch, or (by_tile) tile `index`, by a whole wave; the same for all its lanes.  A lane looks at a sequence.
 template <int TILE>
@@ -80,8 +85,7 @@ __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan,
   int base = 0;
   for (int s0 = 0; s0 < c.seqs; s0 += 64) {
     if (s0) mine = sequence(s0 + lane);
-    const int reach = min(mine.len, c.capacity), tiles = tiles_of<TILE>(mine, group);
-    const int parts = parts_of(reach, u.span);
+    const int tiles = tiles_of<TILE>(mine, group), parts = parts_of(mine, c, plan, u.span);
     int count = by_tile ? tiles : tiles * parts, upto = count;
     if (c.seqs > 1)
 #pragma unroll
@@ -99,7 +103,7 @@ __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan,
       const int last = min((u.tile + 1) * TILE, u.s.count * group) - 1;
       const int seen = min(u.limit(last, group), c.capacity);
       const int reach = min(u.s.len, c.capacity);
-      u.own = p > 1 ? ((reach - 1) / p + 64) / 64 * 64 : u.span;     // (at most span, a multiple of 64 as well)
+      u.own = p > 1 ? ((reach - 1) / p + 64) / 64 * 64 : INT32_MAX;  // (at most span, a multiple of 64 as well)
       u.parts = parts_of(seen, u.own);
       // (by tile, the units before it are those of all tiles before it)
       if (by_tile) u.first = t * p;
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
     const int s = s0 + (threadIdx.x & 63);
     if (s < u.seq) {
       const Sequence x = sequence_of(a.c.starts[s], a.c.starts[s + 1], a.c.lens[s], a.c.rows);
-      before += tiles_of<TILE>(x, a.group) * parts_of(min(x.len, a.c.capacity), u.span);
+      before += tiles_of<TILE>(x, a.group) * parts_of(x, a.c, a.plan, u.span);
     }
   }
 #pragma unroll
@@ -925,13 +929,13 @@ constexpr int64_t PART_BYTES = int64_t(60) << 20;
 // are as many, nothing is cut (64 sequences of 1024, 8 kv heads of 128, bf16: 44 us, 53 us cut), and the join is not launched either where the table
 // cannot name more positions than a part has.  Otherwise about `wanted` units are cut: more of them even out ragged sequences, fewer are fewer to join.
 template <class T, int TILE, int D, class Kernel>
-int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
+int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least, int32_t whole) {
   // of one kv head, at most: every sequence with new tokens may end inside a tile
   const int64_t ends = a.c.seqs < a.c.rows ? a.c.seqs : a.c.rows, tiles = ((int64_t)a.c.rows * a.group + ends * (TILE - 1)) / TILE;
   const int64_t slot = (int64_t)TILE * (D + 2) * sizeof(float) * a.kv_heads;
   const int64_t cus = num_cus();
   int64_t target = 0;
-  if (tiles * a.kv_heads < 2 * cus && a.c.capacity > least) {
+  if (tiles * a.kv_heads < 2 * cus && a.c.capacity > whole) {
     target = cdiv(wanted, a.kv_heads);
     if ((tiles + target) * slot > PART_BYTES) target = PART_BYTES / slot - tiles;
     if (target < 1) target = 0;
@@ -939,6 +943,7 @@ int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least) {
   if (target > 0) {
     a.plan.target = (int32_t)target;
     a.plan.least = least;
+    a.plan.whole = whole;
     a.plan.parts = (float *)scratch((size_t)((tiles + target) * slot));
     if (!a.plan.parts) return fail(AH_ERR_OOM, "ah_paged_attention: no scratch for the parts of long sequences");
   }
@@ -960,15 +965,17 @@ int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
   // and 19.6); at 48, 60 and 44 us; at 256, 182 and 74.  The other way, 16 columns: 35 and 39 us.
   const bool rows = (int64_t)a.c.rows * a.group > (int64_t)32 * a.c.seqs;
   const int64_t cus = num_cus();
-  // Units wanted, of keys: three to a compute unit, 246 us at 32 ragged sequences of up to 32768 positions; two, 277; four, 260.
-  // Least parts: of 128 positions in place of 256, one token after 256 positions takes 9.8 us, not 7.8 (bf16, 8 kv heads of 128), for the join; rows,
-  // whose units are longer, gain by it: 12 tokens after 512, 13.9 us against 18.7 with 256.
+  // Units wanted, of keys: three to a compute unit, 246 us at 24 ragged sequences of up to 24000 positions (8 kv heads of 128, bf16), two, 276, four, 245; at
+  // four equal ones of 8192, 36, 31 and 36.
+  // A part has 256 positions at least, and what has no more than 512 is not cut: 500 positions of 12 heads of 64, bf16, 8.7 us, in two parts, which have to be
+  // joined, 10.0; 1000 in four, 10.1, in two 12.4.  fp32 heads of more than 64 are slower to get through: 500 whole, 20.9, in two parts 17.0.
+  // Rows, whose units are longer, are cut down to 128: 12 tokens after 500 (8 kv heads of 128), 13.9 us against 18.7 with 256.
   if (bf16_pages) {
-    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 3 * cus, 256);
-    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128);
+    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 3 * cus, 256, 512);
+    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128, 128);
   }
-  if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, 3 * cus, 256);
-  return attend<float, 32, D>(a, k_paged_f32<D, 2>, 3 * cus, 256);
+  if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, 3 * cus, 256, D <= 64 ? 512 : 256);
+  return attend<float, 32, D>(a, k_paged_f32<D, 2>, 3 * cus, 256, D <= 64 ? 512 : 256);
 }
 
 }  // namespace
