@@ -60,7 +60,7 @@ def test_infinite_values_reach_those_who_see_them_and_nobody_else(B, dev, dtype,
     with np.errstate(invalid="ignore"):
         for r in range(new):
             extra = np.zeros(D)
-            for p, f, x in put:
+            for (p, f), x in {(p, f): x for p, f, x in put}.items():        # (of two put in one place the later one lies there)
                 if p <= first + r:
                     extra[f] += x
             for h in range(heads):
