@@ -245,6 +245,8 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
 // lane % 16.  Those are, as they lie, the B operand of O^T[16 features, 16 columns] += V^T P^T when its slot 8 g + 4 i + r is taken to mean that
 // position; the A operand is read from V's tile in the same order (ds_read_b64_tr_b16 of four rows).  K goes from the pages straight into its operand's
 // registers (16 rows of 64 bytes to an instruction), V through LDS that is the wave's own, so that no wave waits for another before the end.
+// Bound by the pages: a token each of 24 sequences of up to 24000 positions, 32 heads of 128 on 8, 246 us, 5.0 TB/s; of one sequence of 777, 12 heads of 64, by the
+// loads that wait for each other (lengths, table, page) and the two launches: 10.1 us, 7.2 and 3.7 of them in the kernels.
 template <int D> struct KeysTile {
   static constexpr int PITCH = D + 16, V_BYTES = 32 * PITCH * 2, O_PITCH = D + 4, O_BYTES = 16 * O_PITCH * 4;
   static constexpr int WAVE_BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
@@ -692,7 +694,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // The waves take tiles in turn and are joined, for NC = 1 block of columns (keys) and for 2 (rows): no wave waits for another before the end, and
 // each piece of a page is read once by a workgroup.  With 32 columns to a wave, each streaming all positions, a batch of prompts of 12 heads of 64
 // took 254 us; with the positions cut, 168, and with one block as long, but chunks of 512 in 4096 positions, 16 heads of 64: 398 us, two 369 (88 TFLOP/s of
-// the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.
+// the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.  As it stands, lengths and
+// wave numbers in scalar registers: 148, 344 (94 TFLOP/s), 796; the matrix pipes are busy half of the time.  One token each: a batch of 20 of up to 512
+// positions, 8 heads of 48, 14 us, the loads that wait for each other; 12 of 8192, 32 heads of 128 on 8, 150 us, 5.4 TB/s.
 template <int D, int NC>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;

@@ -7,6 +7,10 @@
 // index.  Where no nucleus is asked for the walk is by index: sums of runs of 64 vectors, a scan over those, and the one run again.
 // With a small top_k all of that happens in the list of the few candidates that the threads' maxima leave.
 //
+// Bound by one workgroup's passes over its row, from the second on out of the caches, and by what a pass does with a logit: a weight takes a dozen 64-bit
+// operations, a bin an addition in LDS.  One row of 50304, top_k 40, 15 us; largest alone 6.5, by index without cuts 24, nucleus 35.  20 rows of 4096, nucleus,
+// 16 us.  160 rows of 131072 in bf16: largest 13 us, by index 52, nucleus 84, all of it mixed 100 (the 42 MB alone 9).  20 of 300, by index, 6.8.
+//
 // Weights are whole numbers of 2^-43 of the largest, so sums are exact and the same in every order.  2^(y/256) for whole y is read from a table, the
 // rest is e^g with |g| <= 2^-9.5: 1 + g + g^2 (1/2 + g/6 + g^2/24), the parentheses in 32 bits (2^-43 of the result), all else in 64.
 #include "common.h"
@@ -29,9 +33,11 @@ constexpr int BINS = 2048, LIST = 2048, STEPS = 256, MOST_WAVES = 16;
 static_assert(BINS == LIST, "as many bins as entries to a thread");
 constexpr int MAX_VOCAB = 1 << 20;              // sums of as many weights of 2^43 stay below 2^63
 constexpr double UNIT = 0x1p43;
-constexpr int FEW = 256;                         // a top_k up to this goes through the maxima of 512 threads or more, which leave about k candidates
-constexpr int LONG = 16384;                      // rows past this have 1024 threads
-constexpr int SMALL = 512;                       // rows up to this are a list from the start
+// A top_k up to this goes through the maxima of 512 threads or more, which leave about k candidates: of 300 logits the first 40 take 9.6 us, by the bins' counts
+// 12.7; of 4096 9.5 and 14.4; of 50304 15.7 and 33.
+constexpr int FEW = 256;
+// Rows past this have 1024 threads: 20 of 8192, nucleus, 17.6 us, with 1024 threads 18.1; of 12000, 21.2 and 19.8; of 32768, 33 and 28; of 4096, 16.3 and 17.5.
+constexpr int LONG = 8192;
 
 // f32 -> whole numbers of the same order, -0 as 0; back
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -395,30 +401,26 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs a) {
   };
 
   auto choose = [&] {
-    const bool small = row.V <= SMALL;
-    if (small || (cut && k <= FEW)) {
-      if (small) row.hits(bound, top, INFINITY, -INFINITY, [&](float l, int index) { list(0, l, index); });
-      else {
-        // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
-        float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
-        block_bounds<THREADS>(lowest, dummy, s);
-        const Bins bin(lowest, top, INFINITY);
-        for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
-        __syncthreads();
-        if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
-        __syncthreads();
-        const bool every = sum_bins<THREADS>(s, 0) < (uint64_t)k;  // fewer maxima than that: all of the row are candidates
-        find_bin<THREADS>(s, 0, 0, (uint64_t)k);
-        const int last = every ? BINS - 1 : same(s.found);
-        float lo = bound, hi;
-        if (last < BINS - 1) bin.around(last, bound, lo, hi);      // (the last bin has no end)
-        row.hits(lo, top, INFINITY, -INFINITY, [&](float l, int index) { if (bin(l) <= last) list(0, l, index); });
-      }
+    if (cut && k <= FEW) {
+      // At least k logits are in the bins (of the threads' maxima) up to the one in which the k-th largest of the maxima lies: those are the candidates.
+      float lowest = mine > -INFINITY ? mine : INFINITY, dummy = mine;
+      block_bounds<THREADS>(lowest, dummy, s);
+      const Bins bin(lowest, top, INFINITY);
+      for (int i = t; i < BINS; i += THREADS) s.bins[0][i] = 0;
+      __syncthreads();
+      if (mine > -INFINITY) atomicAdd((unsigned long long *)&s.bins[0][bin(mine)], 1ull);
+      __syncthreads();
+      const bool every = sum_bins<THREADS>(s, 0) < (uint64_t)k;  // fewer maxima than that: all of the row are candidates
+      find_bin<THREADS>(s, 0, 0, (uint64_t)k);
+      const int last = every ? BINS - 1 : same(s.found);
+      float lo = bound, hi;
+      if (last < BINS - 1) bin.around(last, bound, lo, hi);      // (the last bin has no end)
+      row.hits(lo, top, INFINITY, -INFINITY, [&](float l, int index) { if (bin(l) <= last) list(0, l, index); });
       __syncthreads();
       const int n = same(s.listed[0]);
       if (n <= LIST) {
         sort_list<THREADS>(s, s.list[0], n);
-        const uint32_t kth = cut && n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u, lowest = max(kth, order_of(bound));
+        const uint32_t kth = n > k ? (uint32_t)(same(s.sorted[k - 1]) >> 32) : 0u, lowest = max(kth, order_of(bound));
         if (n <= 64) {                           // a wave alone
           if (wave) return;
           const uint64_t e = lane < n ? s.sorted[lane] : 0;

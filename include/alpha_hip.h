@@ -500,8 +500,10 @@ int32_t ah_decode_next_ticks(int32_t ticks);
  *      table, starts and lens are read when the kernels run, so a captured graph follows what is written there.  What they hold is
  *      checked there too, and nothing outside the arrays is touched: starts are taken into 0 .. rows; a position whose page is
  *      outside 0 .. pages - 1 or past the table is not written, and attention that reads it gives NaN (output and lse).
- *      A page may be shared by sequences; two new tokens must not fall on one row of a page.
- *      All pointers 16-byte aligned (table, starts, lens, lse: 4), strides multiples of 16 bytes; head_dim a multiple of 8 from 8 to 128. ---- */
+ *      A page may be shared by sequences; two new tokens must not fall on one row of a page, and starts must not fall.
+ *      All pointers 16-byte aligned (table, starts, lens, lse: 4), strides multiples of 16 bytes and below 2^31 times 16 bytes; head_dim a
+ *      multiple of 8 from 8 to 128.  Positions from 0x7fff0000 on count as past the table.
+ *      Attention leaves parts of long contexts in the library's scratch, so it belongs on the main stream like all that uses that. ---- */
 typedef struct {
   int32_t dtype;                 /* AH_F32 or AH_BF16: of the pages and of every q, k, v and o that meets them */
   int32_t kv_heads, head_dim;
@@ -550,7 +552,7 @@ int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *a);
  * Sums are taken in 64-bit whole numbers: the same row gives the same token in every batch. */
 typedef struct {
   int32_t dtype;                 /* of the logits: AH_F32 or AH_BF16 */
-  int32_t vocab;
+  int32_t vocab;                 /* 1 .. 2^20 */
   int64_t rows, ld;              /* row stride in elements, at least vocab */
   ah_ptr  logits;
   ah_ptr  temperature;           /* f32 [rows]; 0: 1 */
