@@ -186,6 +186,32 @@ struct SplitTile {                          // D = 32 or 64
 // 309 / 888 -> 262 / 736), 32 x 128 x 32 8.5 / 42 ->
 // 7.3 / 34, 12 x 500 x 64 22 / 184 -> 20 / 140.  Results against 64 bits (4 x 256 x 32 and 4 x 512 x 64): the same without a cap, up to 46 %
 // closer with one of 5 or 30; under a cap of 0.75 with nearly every score at it, dQ up to 12 % further off and down to 13 % closer.
+// tanh in the form of Cephes' tanhf (Moshier): for |x| < TANH_SMALL x + x^3 P(x^2), P here the fifth-order polynomial of least relative error
+// there (fitted by reweighted least squares, Lawson's method), beyond that 1 - 2 / (exp(2 |x|) + 1).  Last places off at most, over all
+// values from 0.5 to 1: 0.73 and 1.63 (the library's tanhf 0.78 and 1.39; its two-part argument and a corrected exponential bring the
+// second to 1.56 and cost 5 % of the forward pass where scores are large).
+constexpr float TANH_SMALL = 0.625f, LOG2E = 1.44269502162933349609375f, LOG2E_REST = 1.925963033e-8f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float z = x * x;
+  float p = -0.005704985465854406f;
+  p = __builtin_fmaf(p, z, 0.02063908614218235f);
+  p = __builtin_fmaf(p, z, -0.05373971536755562f);
+  p = __builtin_fmaf(p, z, 0.13331441581249237f);
+  p = __builtin_fmaf(p, z, -0.3333328068256378f);
+  return __builtin_fmaf(x * z, p, x);
+}
+// 2^UP exp x, x not much above 0 and not below -1e9 (there, as for infinite x, NaN or infinity may come of it): the integer part of
+// x log2 e, whose constant is held in two parts (Cody and Waite), goes into the exponent, 2 to the rest is the instruction's.  0.96 last
+// places off at most, 0.306 root mean square (expf: 0.84, 0.300; a single exponential of x log2 e times what that rounds off: 1.25, 0.41).
+template <int UP>
+__device__ __forceinline__ float exp_of(float x) {
+  const float n = __builtin_rintf(x * LOG2E), rest = __builtin_fmaf(x, LOG2E_REST, __builtin_fmaf(x, LOG2E, -n));
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(rest), (int)n + UP);
+}
+__device__ __forceinline__ float tanh_large(float x) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.0f * LOG2E));
+  return copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f), x);
+}
 // Raw scores (times 2^48) scaled back by `factor` (split_cap_factor) and, with a cap, put through tanh: a score is cap times that
 __device__ __forceinline__ void scores_tanh(f32x16 &s, float cap, float factor) {
 #pragma clang fp contract(off)

@@ -15,6 +15,7 @@ template <int D> struct Geo {
   static constexpr int CHUNKS = ST * D / 8 / 256;      // 16-byte chunks per thread per tile (D=32: 1, 64: 2, 128: 4)
 };
 
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float FIXED_MAX_CAP = 40.f;      // soft caps up to this use the constant-maximum softmax
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }

@@ -697,6 +697,18 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.  As it stands, lengths and
 // wave numbers in scalar registers: 148, 344 (94 TFLOP/s), 796; the matrix pipes are busy half of the time.  One token each: a batch of 20 of up to 512
 // positions, 8 heads of 48, 14 us, the loads that wait for each other; 12 of 8192, 32 heads of 128 on 8, 150 us, 5.4 TB/s.
+// The cap's tanh, as in attention.hip (where the polynomial's origin and both errors stand): up to 0.625, and beyond
+constexpr float TANH_SMALL = 0.625f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float z = x * x;
+  float p = -0.005704985465854406f;
+  p = fmaf(p, z, 0.02063908614218235f);
+  p = fmaf(p, z, -0.05373971536755562f);
+  p = fmaf(p, z, 0.13331441581249237f);
+  p = fmaf(p, z, -0.3333328068256378f);
+  return fmaf(x * z, p, x);
+}
+__device__ __forceinline__ float tanh_large(float x) { return copysignf(fmaf(-2.0f, rcp_fast(exp2_fast(fabsf(x) * (2.0f * LOG2E)) + 1.0f), 1.0f), x); }
 template <int D, int NC>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
