@@ -240,6 +240,22 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
   if (f == 0 && a.lse) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : fmaf(m, LN2, logf(l));
 }
 
+// ------------------------------------------------------------------------------------------ the cap
+// tanh as in attention.hip (where the polynomial's origin and both errors stand): up to 0.625, and beyond.  A last place of the cap is one of the score, whatever
+// the score is, if tanh is 1 - 2 / (e^(2 x) + 1) throughout: the bf16 kernels take that up to FIXED_MAX_CAP, where it is 4e-6, and this above.
+constexpr float TANH_SMALL = 0.625f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float z = x * x;
+  float p = -0.005704985465854406f;
+  p = fmaf(p, z, 0.02063908614218235f);
+  p = fmaf(p, z, -0.05373971536755562f);
+  p = fmaf(p, z, 0.13331441581249237f);
+  p = fmaf(p, z, -0.3333328068256378f);
+  return fmaf(x * z, p, x);
+}
+__device__ __forceinline__ float tanh_large(float x) { return copysignf(fmaf(-2.0f, rcp_fast(exp2_fast(fabsf(x) * (2.0f * LOG2E)) + 1.0f), 1.0f), x); }
+__device__ __forceinline__ float tanh_any(float x) { return fabsf(x) < TANH_SMALL ? tanh_small(x) : tanh_large(x); }
+
 // ------------------------------------------------------------------------------------------ keys, bf16
 // v_mfma_f32_16x16x32_bf16: S^T[32 positions, 16 columns] = K Q^T in two halves of 16, a lane holding positions 16 i + 4 g + r (g = lane / 16, r < 4) of column
 // lane % 16.  Those are, as they lie, the B operand of O^T[16 features, 16 columns] += V^T P^T when its slot 8 g + 4 i + r is taken to mean that
@@ -252,7 +268,7 @@ template <int D> struct KeysTile {
   static constexpr int WAVE_BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
 };
 
-template <int D, bool CAPPED>
+template <int D, int MODE>                       // 0: no cap; 1: one up to FIXED_MAX_CAP; 2: a larger one
 __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
   using G = KeysTile<D>;
   constexpr int KS = D / 32, DB = D / 16, NV = D / 16, TILE = 16;
@@ -282,8 +298,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
       q[ks] = __builtin_bit_cast(bf16x8, x);
     }
   }
-  // CAPPED: e^(2 x / cap) = 2^(c1 s), and the score in base 2 is c2 - 2 c2 / (that + 1); otherwise it is c1 s
-  const float c1 = CAPPED ? 2.0f * a.scale * LOG2E / a.cap : a.scale * LOG2E, c2 = a.cap * LOG2E;
+  // MODE 1: e^(2 x / cap) = 2^(c1 s), and the score in base 2 is c2 - 2 c2 / (that + 1); 2: it is c2 tanh(c1 s); 0: c1 s
+  const float c1 = MODE == 1 ? 2.0f * a.scale * LOG2E / a.cap : MODE == 2 ? a.scale / a.cap : a.scale * LOG2E, c2 = a.cap * LOG2E;
   f32x4 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -337,7 +353,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) s[h][r] = CAPPED ? fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[h][r] * c1) + 1.0f), c2) : s[h][r] * c1;
+      for (int r = 0; r < 4; r++) s[h][r] = MODE == 1 ? fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[h][r] * c1) + 1.0f), c2) : MODE == 2 ? c2 * tanh_any(s[h][r] * c1) : s[h][r] * c1;
     const bool edge = base + 32 > min(least, end);
     if (edge) {
       keep_branch();
@@ -488,9 +504,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   const int limit = i < columns ? min(u.limit(i, a.group), end) : 0;          // positions that the column sees of these
   const uint16_t *K = (const uint16_t *)a.k + head * a.c.head_stride, *V = (const uint16_t *)a.v + head * a.c.head_stride;
   const int32_t *table = a.c.table + (int64_t)u.seq * a.c.table_pages;
-  // MODE 0: the score in base 2 is c1 s, c1 >= 0 (a negative scale turns q's sign).  Capped: e^(2 x / cap) = 2^(c1 s), the score is c2 - 2 c2 / (that + 1)
-  const float c1 = (MODE ? 2.0f * a.scale / a.cap : fabsf(a.scale)) * LOG2E, c2 = a.cap * LOG2E;
-  const float ic2 = MODE ? -1.0f / (2.0f * c2) : 0.f;                         // and 2^(-2 c2 r) with -2 c2 r = 1 / ((e + 1) ic2)
+  // MODE 0: the score in base 2 is c1 s, c1 > 0 (a negative scale turns q's sign; a masked s, -infinity, times a scale of 0 would be NaN).  1: e^(2 x / cap) = 2^(c1 s), the score is c2 - 2 c2 / (that + 1);
+  // 2: c2 tanh(c1 s)
+  const float c1 = MODE == 1 ? 2.0f * a.scale * LOG2E / a.cap : MODE == 2 ? a.scale / a.cap : fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f), c2 = a.cap * LOG2E;
+  const float ic2 = MODE == 1 ? -1.0f / (2.0f * c2) : 0.f;                    // and 2^(-2 c2 r) with -2 c2 r = 1 / ((e + 1) ic2)
   const float slope = MODE ? 1.f : c1;
 
   bf16x8 qf[KS];
@@ -601,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
-          for (int e = 0; e < 16; e++) s[b][e] = fmaf(-2.0f * c2, rcp_fast(exp2_fast(s[b][e] * c1) + 1.0f), c2);
+          for (int e = 0; e < 16; e++) s[b][e] = c2 * tanh_any(s[b][e] * c1);
       }
       if (edge) {
         keep_branch();
@@ -697,18 +714,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.  As it stands, lengths and
 // wave numbers in scalar registers: 148, 344 (94 TFLOP/s), 796; the matrix pipes are busy half of the time.  One token each: a batch of 20 of up to 512
 // positions, 8 heads of 48, 14 us, the loads that wait for each other; 12 of 8192, 32 heads of 128 on 8, 150 us, 5.4 TB/s.
-// The cap's tanh, as in attention.hip (where the polynomial's origin and both errors stand): up to 0.625, and beyond
-constexpr float TANH_SMALL = 0.625f;
-__device__ __forceinline__ float tanh_small(float x) {
-  const float z = x * x;
-  float p = -0.005704985465854406f;
-  p = fmaf(p, z, 0.02063908614218235f);
-  p = fmaf(p, z, -0.05373971536755562f);
-  p = fmaf(p, z, 0.13331441581249237f);
-  p = fmaf(p, z, -0.3333328068256378f);
-  return fmaf(x * z, p, x);
-}
-__device__ __forceinline__ float tanh_large(float x) { return copysignf(fmaf(-2.0f, rcp_fast(exp2_fast(fabsf(x) * (2.0f * LOG2E)) + 1.0f), 1.0f), x); }
 template <int D, int NC>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
@@ -987,7 +992,7 @@ int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
   // joined, 10.0; 1000 in four, 10.1, in two 12.4.  fp32 heads of more than 64 are slower to get through: 500 whole, 20.9, in two parts 17.0.
   // Rows, whose units are longer, are cut down to 128: 12 tokens after 500 (8 kv heads of 128), 13.9 us against 18.7 with 256.
   if (bf16_pages) {
-    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > 0.f ? k_paged_keys_bf16<D, true> : k_paged_keys_bf16<D, false>, 3 * cus, 256, 512);
+    if (!rows) return attend<uint16_t, 16, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_keys_bf16<D, 2> : a.cap > 0.f ? k_paged_keys_bf16<D, 1> : k_paged_keys_bf16<D, 0>, 3 * cus, 256, 512);
     return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128, 128);
   }
   if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, 3 * cus, 256, D <= 64 ? 512 : 256);
@@ -1012,7 +1017,8 @@ extern "C" int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *
   a.k = dp<void>(p->k); a.v = dp<void>(p->v); a.q = dp<void>(d->q); a.o = dp<void>(d->o); a.lse = dp<float>(d->lse);
   a.q_st = d->q_st; a.q_sh = d->q_sh; a.o_st = d->o_st; a.o_sh = d->o_sh;
   a.heads = d->heads; a.kv_heads = p->kv_heads; a.group = d->heads / p->kv_heads; a.head_dim = p->head_dim;
-  a.scale = d->scale; a.cap = d->soft_cap;
+  a.scale = d->scale;
+  a.cap = d->soft_cap < 0x1p40f ? d->soft_cap : 0.f;                 // (a score would have to pass 2^28 for such a cap to move it by its last place)
   const bool bf16_pages = p->dtype == AH_BF16;
   return p->head_dim <= 32 ? attend_sized<32>(a, bf16_pages) : p->head_dim <= 64 ? attend_sized<64>(a, bf16_pages) : attend_sized<128>(a, bf16_pages);
 }

@@ -216,7 +216,7 @@ class PagedContext:
         """Of the next layer (gptBlocks asks for each in turn): the new tokens' keys and values go into its pages, their queries over them."""
         pages = self.pages.pop(0)
         self.backend.pagedAppend(pages, qkv.data, nHead)
-        r = self.backend.pagedAttention(pages, qkv.data, nHead, scale, softCap)
+        r = self.backend.pagedAttention(pages, qkv.data, nHead, scale, max(softCap, 0.0))
         out = Variable(r["output"], False)
         ctx.tape.record(out, [], None)
         return out

@@ -80,3 +80,37 @@ def test_infinite_values_reach_those_who_see_them_and_nobody_else(B, dev, dtype,
     fine = np.isfinite(out)
     h = 2.0 ** -8 if dtype == ffi.BF16 else 0.0
     assert np.all(abs(out - again)[fine] <= (2 * h + 400 * 2.0 ** -24) * np.maximum(abs(again[fine]), 4.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [[1, 3, 1], [40, 3, 70]])
+@pytest.mark.parametrize("scale,cap", [(-0.2, 0.0), (-0.3, 20.0), (-0.3, 90.0), (0.0, 0.0), (0.0, 5.0), (0.2, 41.0), (3.0, 60.0), (3.0, 0.0)])
+def test_scales_of_every_sign_and_size(B, dev, dtype, news, scale, cap):
+    c = Case(dtype, 4, 2, 64, 16, [120, 60, 90], news, seed=5)
+    check_attention(c, *run_attention(B, dev, c, scale, cap), scale, cap)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [[1, 3, 1], [40, 3, 70]])
+@pytest.mark.parametrize("cap", [50.0, 3000.0, 1e7, 2.0 ** 45])
+def test_a_large_cap_costs_no_last_places_of_its_own(B, dev, dtype, news, cap):
+    """The bound of tests/test_gpu_paged.py with the cap's share relative to the score: tanh to 1.63 last places (3.3 u), its argument and the product with the cap, u each
+    (scores here are below half the cap, where a relative error of the argument is no larger in tanh): 6 u |s| in place of 8 u cap."""
+    c, scale = Case(dtype, 4, 2, 64, 16, [120, 60, 90], news, seed=6), 0.2
+    out, lse = run_attention(B, dev, c, scale, cap)
+    q, h, u = c.part("q"), 2.0 ** -8 if dtype == ffi.BF16 else 0.0, 2.0 ** -24
+    for s, length in enumerate(c.lens):
+        k, v = (c.seen(name, s, np.arange(length)) for name in "kv")
+        for r in range(int(c.starts[s]), int(c.starts[s + 1])):
+            n = length - c.news[s] + r - int(c.starts[s]) + 1
+            for head in range(4):
+                raw = scale * (k[:n, head // 2] @ q[r, head])
+                x, size = cap * np.tanh(raw / cap), scale * (abs(k[:n, head // 2]) @ abs(q[r, head]))
+                assert abs(raw).max() < cap / 2
+                e = float(((c.D + 3) * u * size + 10 * u * abs(x)).max())
+                w = np.exp(x - x.max())
+                want, around = (w @ v[:n, head // 2]) / w.sum(), (w @ abs(v[:n, head // 2])) / w.sum()
+                bound = (math.expm1(2 * e + 4 * u) + (n + 16) * u + 2 * h * (1 + h)) * around * (1 + h) + (h + 2 * u) * abs(want)
+                assert np.all(abs(values(out[r]).reshape(4, 64)[head] - want) <= bound), (s, r, head)
+                want_l = x.max() + math.log(w.sum())
+                assert abs(lse[r, head] - want_l) <= e + (n + 16) * u + 4 * u * abs(want_l) + 8 * u, (s, r, head)
