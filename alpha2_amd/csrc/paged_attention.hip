@@ -713,9 +713,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 // took 254 us; with the positions cut, 168, and with one block as long, but chunks of 512 in 4096 positions, 16 heads of 64: 398 us, two 369 (88 TFLOP/s of
 // the 154 that fp32 products reach; the exponentials and the loads' addresses are in the way); heads of 128: 1144 and 972.  As it stands, lengths and
 // wave numbers in scalar registers: 148, 344 (94 TFLOP/s), 796; the matrix pipes are busy half of the time.  One token each: a batch of 20 of up to 512
-// positions, 8 heads of 48, 14 us, the loads that wait for each other; 12 of 8192, 32 heads of 128 on 8, 150 us, 5.4 TB/s.
+// positions, 8 heads of 48, 14 us, the loads that wait for each other; 40 of 5000, 32 heads of 128 on 8, 286 us, 5.7 TB/s (with one workgroup to a compute unit, which 256 registers and more would mean, 4 of 8192 take
+// 63 us, not 55).
 template <int D, int NC>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_paged_f32(AttendArgs a) {
+__global__ __launch_bounds__(256, D <= 64 || NC == 1 ? 2 : 1) void k_paged_f32(AttendArgs a) {
   constexpr int KQ = D / 16, W = D >= 64 ? 4 : 2, VH = D / (16 * W), DB = D / 16, TILE = 16 * NC, O_PITCH = D + 4;
   __shared__ __attribute__((aligned(16))) float joined[4 * TILE * O_PITCH];
   __shared__ float tops[4][TILE], sums[4][TILE];
@@ -988,6 +989,7 @@ int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
   const int64_t cus = num_cus();
   // Units wanted, of keys: three to a compute unit, 246 us at 24 ragged sequences of up to 24000 positions (8 kv heads of 128, bf16), two, 276, four, 245; at
   // four equal ones of 8192, 36, 31 and 36.
+  // fp32 heads of more than 64, two workgroups to a compute unit as well: 4 of 8192 (8 kv heads) 61 us with three, 55 with four, 3 of 24000 (16) 226 and 203.
   // A part has 256 positions at least, and what has no more than 512 is not cut: 500 positions of 12 heads of 64, bf16, 8.7 us, in two parts, which have to be
   // joined, 10.0; 1000 in four, 10.1, in two 12.4.  fp32 heads of more than 64 are slower to get through: 500 whole, 20.9, in two parts 17.0.
   // Rows, whose units are longer, are cut down to 128: 12 tokens after 500 (8 kv heads of 128), 13.9 us against 18.7 with 256.
@@ -995,7 +997,7 @@ int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
     if (!rows) return attend<uint16_t, 16, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_keys_bf16<D, 2> : a.cap > 0.f ? k_paged_keys_bf16<D, 1> : k_paged_keys_bf16<D, 0>, 3 * cus, 256, 512);
     return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128, 128);
   }
-  if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, 3 * cus, 256, D <= 64 ? 512 : 256);
+  if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, (D <= 64 ? 3 : 4) * cus, 256, D <= 64 ? 512 : 256);
   return attend<float, 32, D>(a, k_paged_f32<D, 2>, 3 * cus, 256, D <= 64 ? 512 : 256);
 }
 
