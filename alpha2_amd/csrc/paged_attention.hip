@@ -184,6 +184,8 @@ constexpr float LN2 = 0.693147180559945309f;
 
 // Joins the parts of a tile: a thread to four features of a column.  Few columns can have many parts: there four waves share them, each its own sum with its
 // own running maximum, and are joined in LDS; a workgroup has 64 such fours.  A tile of rows has many columns, and a workgroup 256 fours of it.
+// One sequence of 32768, 8 kv heads of 128, in 96 parts: 35 us with attention, one wave to 64 fours 45; four of 8192, 32 columns each in a tile of 128: 39 us where a
+// workgroup of 256 threads joins a whole tile 63.
 constexpr int join_ways(int tile) { return tile <= 32 ? 4 : 1; }
 constexpr int join_slices(int tile, int d) { return tile * d / 4 * join_ways(tile) / 256; }
 template <class T, int TILE, int D>
@@ -242,7 +244,8 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs a) {
 
 // ------------------------------------------------------------------------------------------ the cap
 // tanh as in attention.hip (where the polynomial's origin and both errors stand): up to 0.625, and beyond.  A last place of the cap is one of the score, whatever
-// the score is, if tanh is 1 - 2 / (e^(2 x) + 1) throughout: the bf16 kernels take that up to FIXED_MAX_CAP, where it is 4e-6, and this above.
+// the score is, if tanh is 1 - 2 / (e^(2 x) + 1) throughout: the bf16 kernels take that up to FIXED_MAX_CAP, where it is 4e-6, and this above.  Chunks of 1024 in
+// 8192, 32 heads of 128 on 8: the one 341 us, the other 432; 16 heads of 64, 144 and 188; a token each of 16 sequences of 8192, 122 and 123, of 8 of 1000, 13.5 and 13.9.
 constexpr float TANH_SMALL = 0.625f;
 __device__ __forceinline__ float tanh_small(float x) {
   const float z = x * x;
