@@ -8,12 +8,13 @@
 // Work.  The heads that share keys are rows of one matrix: a COLUMN is a (new token, head of the group), column i of a sequence token
 // i / group, head i % group.  A workgroup takes one unit: TILE columns of a sequence, one kv head, one part of the positions.  Which unit that is
 // follows from starts and lens on the device (find_unit), so the lengths need not be known on the host, ragged batches are cut evenly
-// (parts are of one length for the whole launch, about the launch's work over the workgroups wanted) and a captured launch follows them.
+// (parts are as long as the launch's work over the workgroups wanted, and those of a sequence as long as each other) and a captured launch follows them.
 //
 // Two kernels for each type; both compute every case, which is taken is a matter of speed (ah_paged_attention):
 //   keys   16 columns; the four waves take tiles of positions in turn and are joined in LDS.  For one or a few new tokens a sequence, where the
 //          launch is bound by reading the pages once: 16 columns are the fewest that the matrix instructions take, most of them idle for one token.
-//   rows   the waves own columns and stream the same positions.  For chunks and prompts, bound by the matrix and vector pipes.
+//   rows   bf16: 128 columns, the waves own 32 each and stream the same positions through LDS; fp32: 32 columns, otherwise as keys.  For chunks and
+//          prompts, bound by the matrix and vector pipes.
 //
 // Masked places.  A position past a column's limit has its score replaced by -infinity, whatever it was.  Its value would still meet a weight of 0
 // in the matrix product, and 0 x infinity is NaN; so rows past the part's end are zeros, and where some columns see a row that others do
