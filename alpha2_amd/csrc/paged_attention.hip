@@ -471,8 +471,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_keys_bf16(AttendArgs a) {
 // (by the lane that fetches them), so that 16 rows' same piece and four rows' same 64 bytes each meet all 64 banks.
 // The two tiles are arrays of their own, and the loop is written out for both: an LDS read that may touch what a load under way writes waits for it, and
 // the compiler keeps them apart by the array.  Both halves of a tile's scores are taken together, so that the values (whose reads wait all the same) come
-// late.  Two sequences, chunks of 2048 and 1200 behind 14336 and 5058 positions, 32 heads of 128 on 8: 746 us, 840 TFLOP/s of the 1218 that a large product
-// reaches; one array and a half at a time, 791; the values' finite form chosen in the loop and not in LDS, 989.  Bound by the vector
+// late.  Two sequences, chunks of 2048 and 1200 behind 14336 and 5058 positions, 32 heads of 128 on 8: 702 us, 890 TFLOP/s of the 1218 that a large product
+// reaches; before page and row were the wave's, 746; one array and a half at a time, 791; the values' finite form chosen in the loop and not in LDS, 989.  Bound by the vector
 // instructions of the softmax and by waiting between them and the matrix ones, two waves to a SIMD.
 // MODE 0: no cap; 1: a cap up to 40, whose softmax takes the cap itself for the maximum (attention_bf16.hip); 2: a larger cap.
 typedef __attribute__((address_space(3))) void lds_void;
@@ -489,7 +489,7 @@ template <int D> struct RowsTile {
   }
 };
 
-template <int D, int MODE>
+template <int D, int MODE, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   using G = RowsTile<D>;
   constexpr int DB = D / 32, KS = D / 16, TILE = 128, N = G::LOADS;
@@ -534,9 +534,20 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
 
   // What this lane fetches: piece `lane % PIECES`, as it lands, of row base + its_row(n).  Positions past the end look at the last one's entry, so that nothing
   // here branches: page and row in 16-byte pieces, one multiplication each, and the row of zeros or NaN where they name no place.
+  // WHOLE: pages of a multiple of 64 positions hold whole tiles (which begin at multiples of 64): page and row are the wave's, and a lane has only its place
+  // in the tile to add.
   auto its_row = [&](int n) { return (wave * N + n) * (64 / G::PIECES) + lane / G::PIECES; };
-  uint32_t entry[N], line[N];
+  uint32_t entry[N], line[N], tile_entry = 0, tile_line = 0;
+  uint64_t in_tile[N];
+#pragma unroll
+  for (int n = 0; n < N; n++) in_tile[n] = ((uint64_t)(uint32_t)its_row(n) * a.c.row_pieces + (uint32_t)(lane % G::PIECES ^ G::turned(its_row(n)))) * 16;
   auto entries = [&](int base) {
+    if (WHOLE) {
+      const uint32_t p = (uint32_t)min(base, end - 1), page = quotient(p, a.c.page_rows);
+      tile_entry = (uint32_t)table[page];
+      tile_line = p - page * a.c.page_rows.divisor;
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < N; n++) {
       const uint32_t p = (uint32_t)min(base + its_row(n), end - 1), page = quotient(p, a.c.page_rows);
@@ -546,12 +557,22 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows_bf16(AttendArgs a) {
   };
   const uint32_t pages = (uint32_t)a.c.pages;
   auto load = [&](char *kt, char *vt, int base) {
+    if (WHOLE && base + ST <= end && tile_entry < pages) {
+      const uint64_t at = ((uint64_t)tile_entry * a.c.page_pieces + (uint64_t)tile_line * a.c.row_pieces) * 16;
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        __builtin_amdgcn_global_load_lds((glb_void *)((const char *)K + at + in_tile[n]), (lds_void *)(kt + (wave * N + n) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void *)((const char *)V + at + in_tile[n]), (lds_void *)(vt + (wave * N + n) * 1024), 16, 0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < N; n++) {
       const int r = its_row(n);
+      const uint32_t its_entry = WHOLE ? tile_entry : entry[n], its_line = WHOLE ? tile_line + r : line[n];
       const uint32_t piece = (uint32_t)(lane % G::PIECES ^ G::turned(r));
-      const uint64_t at = (uint64_t)entry[n] * a.c.page_pieces + ((uint64_t)line[n] * a.c.row_pieces + piece);
-      const bool wanted = base + r < end && (int)piece * 8 < a.head_dim, there = entry[n] < pages;
+      const uint64_t at = (uint64_t)its_entry * a.c.page_pieces + ((uint64_t)its_line * a.c.row_pieces + piece);
+      const bool wanted = base + r < end && (int)piece * 8 < a.head_dim, there = its_entry < pages;
       const uint16_t *k = (const uint16_t *)nothing[0], *v = k;
       k = wanted ? there ? K + at * 8 : (const uint16_t *)nothing[1] : k;
       v = wanted && there ? V + at * 8 : v;
@@ -999,7 +1020,13 @@ int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
   // Rows, whose units are longer, are cut down to 128: 12 tokens after 500 (8 kv heads of 128), 13.9 us against 18.7 with 256.
   if (bf16_pages) {
     if (!rows) return attend<uint16_t, 16, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_keys_bf16<D, 2> : a.cap > 0.f ? k_paged_keys_bf16<D, 1> : k_paged_keys_bf16<D, 0>, 3 * cus, 256, 512);
-    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2> : a.cap > 0.f ? k_paged_rows_bf16<D, 1> : k_paged_rows_bf16<D, 0>, 2 * cus, 128, 128);
+    // Tiles inside a page are fetched by the wave's address where a row has 16 pieces and more: chunks of 2048 and 1200, 32 heads of 128, in pages of 64
+    // positions 702 us, position by position 760; heads of 64, the same; of 32, 33 and 31.
+    constexpr bool MANY = D > 64;
+    if (MANY && a.c.page_rows.divisor % ST == 0 && a.head_dim == D)
+      return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2, MANY> : a.cap > 0.f ? k_paged_rows_bf16<D, 1, MANY> : k_paged_rows_bf16<D, 0, MANY>, 2 * cus, 128, 128);
+    return attend<uint16_t, 128, D>(a, a.cap > FIXED_MAX_CAP ? k_paged_rows_bf16<D, 2, false> : a.cap > 0.f ? k_paged_rows_bf16<D, 1, false> : k_paged_rows_bf16<D, 0, false>,
+                                    2 * cus, 128, 128);
   }
   if (!rows) return attend<float, 16, D>(a, k_paged_f32<D, 1>, (D <= 64 ? 3 : 4) * cus, 256, D <= 64 ? 512 : 256);
   return attend<float, 32, D>(a, k_paged_f32<D, 2>, 3 * cus, 256, D <= 64 ? 512 : 256);

@@ -114,3 +114,22 @@ def test_a_large_cap_costs_no_last_places_of_its_own(B, dev, dtype, news, cap):
                 assert np.all(abs(values(out[r]).reshape(4, 64)[head] - want) <= bound), (s, r, head)
                 want_l = x.max() + math.log(w.sum())
                 assert abs(lse[r, head] - want_l) <= e + (n + 16) * u + 4 * u * abs(want_l) + 8 * u, (s, r, head)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0, 60.0])
+@pytest.mark.parametrize("page", [64, 128, 192])
+@pytest.mark.parametrize("heads,kv_heads,lens,news", [(4, 2, [300, 64, 129, 1000], [200, 64, 129, 40]), (2, 1, [63, 65, 2500], [63, 60, 50]), (8, 1, [700, 3, 640], [9, 3, 20])])
+def test_pages_that_hold_whole_tiles(B, dev, cap, page, heads, kv_heads, lens, news):
+    """bf16 heads of 128 in pages of a multiple of 64 positions, whose tiles are fetched by one address: ends inside a tile, at its end, and cut contexts."""
+    c = Case(ffi.BF16, heads, kv_heads, 128, page, lens, news, seed=page + heads, heads_first=page == 128, entries=2)
+    check_attention(c, *run_attention(B, dev, c, 0.09, cap), 0.09, cap)
+
+
+@pytest.mark.parametrize("page", [64, 192])
+def test_missing_pages_that_hold_whole_tiles(B, dev, page):
+    c = Case(ffi.BF16, 4, 2, 128, page, [500, 400, 2100], [100, 90, 40], seed=2, entries=2)
+    c.table[0, 1], c.table[2, 3] = c.pages, -1
+    c.table[1, -(-400 // page):] = 2 ** 31 - 1           # behind what the sequence has: nobody reads them
+    pages = c.upload(dev)
+    c.table = np.where((c.table < 0) | (c.table >= c.pages), 0, c.table).astype(np.int32)
+    check_attention(c, *run_attention(B, dev, c, 0.09, 0.0, pages=pages), 0.09, 0.0, bad={(0, 1), (2, 3)})
