@@ -156,7 +156,7 @@ class PagedContext:
             return None
         if cfg.nEmbd % cfg.nHead or not flashHeadSize(cfg.nEmbd // cfg.nHead) or cfg.vocabSize > 1 << 20 or max(longest) > cfg.blockSize:
             return None
-        if params["wpe"].data.shape[0] < max(longest):
+        if len(params["layers"]) != cfg.nLayer or params["wpe"].data.shape[0] < max(longest):
             return None
         kept = PagedContext(cfg, params, backend, longest)
         try:

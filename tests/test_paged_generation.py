@@ -100,6 +100,13 @@ def test_models_whose_sequences_are_run_one_by_one(monkeypatch, more):
     assert [(a[3], a[5], a[6], a[7]) for a in calls] == [("a", configs[0], "release", "flush"), ("b", configs[1], "release", "flush")]
 
 
+def test_parameters_of_another_model_are_run_one_by_one():
+    cfg, backend = ModelConfig(**CFG), HipBackend.__new__(HipBackend)
+    wpe = lambda rows: type("V", (), {"data": T(rows, 16)})()
+    assert PagedContext.of(cfg, {"layers": [], "wpe": wpe(12)}, backend, [3]) is None
+    assert PagedContext.of(cfg, {"layers": [{}], "wpe": wpe(2)}, backend, [3]) is None
+
+
 def test_more_tokens_than_a_sequence_was_given_room_for():
     kept = PagedContext(ModelConfig(**CFG), {}, None, [3, 12])
     kept.lens[:] = 2, 12
