@@ -996,6 +996,8 @@ class HipBackend:
         return t
 
     def _pages_desc(self, pages: Pages) -> ffi.AhPages:
+        if pages.v.store != pages.k.store:              # (an op that takes f32 alone may have given one of the two f32 storage since)
+            raise TypeError(f"op expects keys and values of one type in the pages, got {pages.k.store} and {pages.v.store}")
         n, positions, heads, D = pages.k.shape
         p = ffi.AhPages()
         p.dtype, p.kv_heads, p.head_dim, p.page_rows, p.pages = ffi.DTYPE_CODE[pages.k.store], heads, D, positions, n

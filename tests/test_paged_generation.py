@@ -68,6 +68,23 @@ def test_tensors_of_another_type(backend):
             backend.pagedAttention(pages(), T(5, 48, store="bf16"), 6, 1.0)
 
 
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_pages_whose_storage_has_changed_since(backend, which):
+    """FastHipBackend's ops that take f32 alone give a bf16 tensor f32 storage in place: keys of one type are not read beside values of another."""
+    def nothing(*a):
+        raise AssertionError("the library has been called")
+    backend.lib = type("Lib", (), {"__getattr__": lambda self, name: nothing})()
+    backend._launch_flash = backend._ptr = lambda *a: 0
+    kept = pages("bf16")
+    getattr(kept, which).store = "f32"
+    new = lambda n: T(5, n, store=kept.k.store)
+    backend._new = lambda shape, dtype="f32", store=None: T(*shape, store=store)
+    with pytest.raises(TypeError, match="one type"):
+        backend._pages_desc(kept)
+    with pytest.raises(TypeError, match="one type"):
+        backend.pagedAppend(kept, new(80), 6)
+
+
 @pytest.mark.parametrize("name,t,error", [("uniform", T(4), ValueError), ("uniform", I(5), TypeError), ("temperature", T(5, 1), ValueError),
                                           ("temperature", T(5, store="bf16"), TypeError), ("topk", T(5), TypeError), ("topk", I(6), ValueError),
                                           ("topp", I(5), TypeError), ("minp", T(1), ValueError)])
