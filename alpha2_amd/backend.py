@@ -24,6 +24,13 @@ from ._ffi import check
 _NP = {"f32": np.float32, "i32": np.int32, "f16": np.uint16, "bf16": np.uint16, "f64": np.float64}
 
 
+def _bf16_bits(x: np.ndarray) -> np.ndarray:
+    """f32 to the nearest bf16, ties to the even one; NaN stays NaN."""
+    u = x.view(np.uint32)
+    near = (u + (0x7FFF + ((u >> 16) & 1))) >> 16
+    return np.where(np.isnan(x), (u >> 16) | 0x40, near).astype(np.uint16)
+
+
 def shapeSize(shape) -> int:
     return math.prod(map(int, shape))
 
@@ -186,14 +193,18 @@ class HipBackend:
         if t._buf is None or not t._dev_valid:
             if not t._host_valid:
                 raise RuntimeError("use of a released tensor")
+            rounded = t.store != t.dtype                        # host contents are f32: stored in bf16, they are read back as that
+            host = _bf16_bits(t._host) if rounded else t._host
             if t._buf is None:
-                t._buf = _Buf(self.lib, t._host.nbytes)
+                t._buf = _Buf(self.lib, host.nbytes)
                 t._off = 0
             t._backend = self
             t._buf.own()
-            if t._host.nbytes:
-                check(self.lib.ah_upload(t._buf.ptr + t._off, t._host.ctypes.data_as(C.c_void_p), t._host.nbytes))
+            if host.nbytes:
+                check(self.lib.ah_upload(t._buf.ptr + t._off, host.ctypes.data_as(C.c_void_p), host.nbytes))
             t._dev_valid = True
+            if rounded:
+                t._host, t._host_valid = None, False
         return t._buf.ptr + t._off
 
     def _download(self, t: TensorData) -> np.ndarray:
