@@ -154,18 +154,22 @@ def sampleTokensBatch(config: ModelConfig, params: dict, backend, rngs: Sequence
         return [sampleTokens(config, params, backend, r, p, c, releaseTensor, flushGpu) for r, p, c in zip(rngs, prompts, configs)]
     tokens = [np.concatenate([p, np.zeros(n - p.size, np.int32)]) for p, n in zip(prompts, wanted)]
     at = [int(p.size) for p in prompts]                                     # tokens known on the host
-    warmth = [1.0 if math.isnan(c.temperature) else c.temperature for c in configs]         # (what selectToken makes of it)
-    topp = [min(1.0, max(0.0, c.topp)) if c.topp is not None and math.isfinite(c.topp) else 1.0 for c in configs]
+    # What selectToken makes of the options, in 32 bits: none is rounded to a number that means something else (a temperature of 0, a
+    # nucleus of nothing or of all, a top_k modulo 2^32).
+    least, most, below_one = 2.0 ** -126, 2.0 ** 127, 1 - 2.0 ** -24
+    warmth = [1.0 if math.isnan(c.temperature) else min(max(c.temperature, least), most) if c.temperature > 0 else 0.0 for c in configs]
+    topk = [min(max(c.topk, 0), config.vocabSize) for c in configs]
+    topp = [min(max(c.topp, least), below_one) if c.topp is not None and 0 < c.topp < 1 else 1.0 for c in configs]
     options, chosen = {}, []
 
     def choose(logits: TensorData, seqs: tuple) -> TensorData:
         if seqs not in options:
             options.clear()
             options[seqs] = [TensorData((len(seqs),), dtype, np.array(list(values))) for dtype, values in (
-                ("f32", (warmth[i] for i in seqs)), ("i32", (configs[i].topk for i in seqs)), ("f32", (topp[i] for i in seqs)))]
+                ("f32", (warmth[i] for i in seqs)), ("i32", (topk[i] for i in seqs)), ("f32", (topp[i] for i in seqs)))]
         # (a draw that f32 would round to 1 stays below it)
         draws = np.array([rngs[i].next() if warmth[i] > 0 else 0.0 for i in seqs]).astype(np.float32)
-        r = backend.sampleRows(logits, TensorData((len(seqs),), "f32", np.minimum(draws, np.float32(1 - 2.0 ** -24))), *options[seqs])
+        r = backend.sampleRows(logits, TensorData((len(seqs),), "f32", np.minimum(draws, np.float32(below_one))), *options[seqs])
         if releaseTensor is not None:
             releaseTensor(logits)
         chosen.append((seqs, r["tokens"]))

@@ -139,3 +139,71 @@ def test_every_sequence_has_pages_of_its_own():
     assert sorted(p for s in owned for p in s) == list(range(sum(need)))
     for i, s in enumerate(owned):
         assert set(kept.table[i].tolist()) == s
+
+
+class OneTokenEach:
+    """In PagedContext's place: logits of nothing; `asked` holds the options that sampleRows was given with each row."""
+    MOST_ROWS = 8192
+
+    def __init__(self):
+        self.asked = []
+
+    def forward(self, seqs, counts, tokens, wanted, release):
+        return T(len(wanted), 20)
+
+    def close(self):
+        pass
+
+    def sampleRows(self, logits, uniform, temperature, topk, topp):
+        self.asked.append([t.data.copy() for t in (uniform, temperature, topk, topp)])
+        return {"tokens": I(logits.shape[0])}
+
+
+class Draw:
+    def __init__(self, *draws):
+        self.draws = list(draws)
+
+    def next(self):
+        return self.draws.pop(0)
+
+
+@pytest.mark.parametrize("config,temperature,topk,topp", [
+    # selectToken: 0 < topP < 1 cuts and walks from the largest down, whatever of it f32 can hold; 0, 1, NaN and what lies outside do not
+    (dict(topp=1 - 1e-12), lambda t: t == np.float32(0.8), lambda k: k == 20 or k == 0, lambda p: 1 - 1e-7 < p < 1),
+    (dict(topp=1e-60), None, None, lambda p: 0 < p < 1e-30),
+    (dict(topp=0.9), None, None, lambda p: p == np.float32(0.9)),
+    (dict(topp=0.0), None, None, lambda p: not 0 < p < 1),
+    (dict(topp=1.0), None, None, lambda p: not 0 < p < 1),
+    (dict(topp=float("nan")), None, None, lambda p: not 0 < p < 1),
+    (dict(topp=None), None, None, lambda p: not 0 < p < 1),
+    # 0 < topk < vocabulary keeps so many; others keep all, those that 32 bits do not hold among them
+    (dict(topk=2 ** 32 + 5), None, lambda k: not 0 < k < 20, None),
+    (dict(topk=2 ** 70), None, lambda k: not 0 < k < 20, None),
+    (dict(topk=-2 ** 70), None, lambda k: not 0 < k < 20, None),
+    (dict(topk=20), None, lambda k: not 0 < k < 20, None),
+    (dict(topk=19), None, lambda k: k == 19, None),
+    # a temperature above 0 samples, 0 and below take the largest, NaN counts as 1
+    (dict(temperature=1e-60), lambda t: 0 < t < 1e-30, None, None),
+    (dict(temperature=1e60), lambda t: 1e30 < t, None, None),
+    (dict(temperature=float("inf")), lambda t: 1e30 < t, None, None),
+    (dict(temperature=float("nan")), lambda t: t == 1, None, None),
+    (dict(temperature=0.0), lambda t: t == 0, None, None),
+    (dict(temperature=-1e-60), lambda t: t <= 0, None, None),
+])
+def test_options_keep_their_side_of_what_switches_them_off(monkeypatch, config, temperature, topk, topp):
+    """SampleConfig's numbers have 64 bits, the kernel's 32: none of them may be rounded to one that means something else."""
+    kept = OneTokenEach()
+    monkeypatch.setattr(sample.PagedContext, "of", staticmethod(lambda *a: kept))
+    with np.errstate(over="raise", invalid="raise"):
+        sampleTokensBatch(ModelConfig(**CFG), {}, kept, [Draw(0.25)], [[1]], SampleConfig(**{"steps": 1, **config}))
+    (_, t, k, p), = kept.asked
+    assert t.dtype == p.dtype == np.float32 and k.dtype == np.int32
+    for got, right in ((t, temperature), (k, topk), (p, topp)):
+        assert right is None or right(got[0]), got[0]
+
+
+def test_draws_stay_below_one(monkeypatch):
+    kept = OneTokenEach()
+    monkeypatch.setattr(sample.PagedContext, "of", staticmethod(lambda *a: kept))
+    sampleTokensBatch(ModelConfig(**CFG), {}, kept, [Draw(1 - 2.0 ** -53), Draw(0.0)], [[1], [2]], SampleConfig(steps=1))
+    assert kept.asked[0][0].tolist() == [1 - 2.0 ** -24, 0.0]
