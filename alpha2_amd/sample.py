@@ -147,7 +147,9 @@ def sampleTokensBatch(config: ModelConfig, params: dict, backend, rngs: Sequence
             raise ValueError(f"prompt of {p.size} tokens, where 1 to blockSize {config.blockSize} are taken")
         if p.min() < 0 or p.max() >= config.vocabSize:
             raise ValueError(f"prompt with tokens outside 0 .. {config.vocabSize - 1}")
-    wanted = [min(p.size + max(c.steps, 0), config.blockSize) for p, c in zip(prompts, configs)]
+    if any(c.steps < 0 for c in configs):
+        raise ValueError(f"steps {[c.steps for c in configs]}, where 0 and more are taken")
+    wanted = [min(p.size + c.steps, config.blockSize) for p, c in zip(prompts, configs)]
     run = [i for i in range(len(prompts)) if wanted[i] > prompts[i].size]
     kept = PagedContext.of(config, params, backend, [wanted[i] for i in run]) if run else None
     if kept is None:

@@ -207,3 +207,15 @@ def test_draws_stay_below_one(monkeypatch):
     monkeypatch.setattr(sample.PagedContext, "of", staticmethod(lambda *a: kept))
     sampleTokensBatch(ModelConfig(**CFG), {}, kept, [Draw(1 - 2.0 ** -53), Draw(0.0)], [[1], [2]], SampleConfig(steps=1))
     assert kept.asked[0][0].tolist() == [1 - 2.0 ** -24, 0.0]
+
+
+def test_fewer_than_no_steps(monkeypatch):
+    """Refused by sampleTokens: here too, whether the sequences are run together or one by one."""
+    with pytest.raises(ValueError):
+        sample.sampleTokens(ModelConfig(**CFG), {}, None, None, [1, 2], SampleConfig(steps=-1))
+    for of in (lambda *a: OneTokenEach(), lambda *a: None):
+        monkeypatch.setattr(sample.PagedContext, "of", staticmethod(of))
+        monkeypatch.setattr(sample, "sampleTokens", lambda *a: np.array(a[4]))
+        for steps in ([-1, 3], [0, -5]):
+            with pytest.raises(ValueError, match="steps"):
+                sampleTokensBatch(ModelConfig(**CFG), {}, OneTokenEach(), [Draw(), Draw(0.1, 0.2, 0.3)], [[1, 2], [3]], [SampleConfig(steps=n) for n in steps])
