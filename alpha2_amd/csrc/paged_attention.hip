@@ -1052,6 +1052,8 @@ extern "C" int32_t ah_paged_attention(const AhPages *p, const AhPagedAttention *
   a.heads = d->heads; a.kv_heads = p->kv_heads; a.group = d->heads / p->kv_heads; a.head_dim = p->head_dim;
   a.scale = d->scale;
   a.cap = d->soft_cap < 0x1p40f ? d->soft_cap : 0.f;                 // (a score would have to pass 2^28 for such a cap to move it by its last place)
+  // Under a cap of 2^-40 scores are 0 to the last place of their exponential; a smaller one's reciprocal may be infinite, and 0 times that NaN.
+  if (a.cap > 0.f && a.cap < 0x1p-40f) a.cap = 0x1p-40f;
   const bool bf16_pages = p->dtype == AH_BF16;
   return p->head_dim <= 32 ? attend_sized<32>(a, bf16_pages) : p->head_dim <= 64 ? attend_sized<64>(a, bf16_pages) : attend_sized<128>(a, bf16_pages);
 }
