@@ -1,5 +1,4 @@
 """Pages and sampling at the ends of what they take: the smallest caps, the largest vocabulary, pages filled from the host, a sequence alone and beside others."""
-
 import numpy as np
 import pytest
 
