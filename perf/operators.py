@@ -13,6 +13,8 @@ append and attend:
 sample:
     dtype, rows, vocab, pick: "greedy", "plain", "topk", "topp", "minp" or "mixed" (each row its own)
 The lengths follow from the case alone; the values, and where the pages lie, from the seed.
+With `own`, run issues its work on the library's stream, which neither waits for torch's nor is waited for by it: prepare ends with what it
+made being there, and whoever reads run's outputs with torch waits for the device first.
 """
 import math
 
@@ -146,12 +148,14 @@ def prepare(case, seed):
         on = {k: (rand[0] * 5).int() == i if mixed else torch.full((rows,), c["pick"] == k, device="cuda")
               for i, k in enumerate(("greedy", "plain", "topk", "topp", "minp"))}
         both = on["topk"] | (on["topp"] & (rand[3] < 0.3) if mixed else on["greedy"])
-        return {"case": dict(c), "logits": logits, "uniform": rand[1].contiguous(),
-                "temperature": torch.where(on["greedy"], off, 0.8 if not mixed else 0.5 + rand[2]),
-                "top_k": torch.where(both, torch.full_like(off, 40.0) if not mixed else 1 + 200 * rand[3], off).int(),
-                "top_p": torch.where(on["topp"], 0.9 if not mixed else 0.5 + 0.49 * rand[4], off + 1),
-                "min_p": torch.where(on["minp"], 0.05 if not mixed else 0.2 * rand[4] + 0.001, off),
-                "tokens": torch.zeros(rows, dtype=torch.int32, device="cuda"), "logprobs": torch.zeros(rows, device="cuda")}
+        s = {"case": dict(c), "logits": logits, "uniform": rand[1].contiguous(),
+             "temperature": torch.where(on["greedy"], off, 0.8 if not mixed else 0.5 + rand[2]),
+             "top_k": torch.where(both, torch.full_like(off, 40.0) if not mixed else 1 + 200 * rand[3], off).int(),
+             "top_p": torch.where(on["topp"], 0.9 if not mixed else 0.5 + 0.49 * rand[4], off + 1),
+             "min_p": torch.where(on["minp"], 0.05 if not mixed else 0.2 * rand[4] + 0.001, off),
+             "tokens": torch.zeros(rows, dtype=torch.int32, device="cuda"), "logprobs": torch.zeros(rows, device="cuda")}
+        torch.cuda.synchronize()
+        return s
 
     lens, news = _lengths(c)
     H, Hk, D, page, seqs = c["heads"], c["kv_heads"], c["size"], c["page"], c["seqs"]
@@ -176,6 +180,7 @@ def prepare(case, seed):
         angles = torch.outer(torch.arange(c["longest"], dtype=torch.float64),
                              10000.0 ** (-2.0 * torch.arange(c["rot"] // 2, dtype=torch.float64) / c["rot"]))
         s["rotary"] = torch.cat([angles.cos(), angles.sin()], 1).float().cuda()
+    torch.cuda.synchronize()
     return s
 
 
