@@ -28,6 +28,12 @@ using namespace ah;
 
 namespace {
 
+template <int D> struct Geo {
+  static constexpr int PITCH = D + 16;                 // bf16 elements; (D+16)*2 bytes = 32 mod 128 for D in {32,64,128}... see tile_frag_t
+  static constexpr int ELEMS = ST * PITCH;
+  static constexpr int CHUNKS = ST * D / 8 / 256;      // 16-byte chunks per thread per tile (D=32: 1, 64: 2, 128: 4)
+};
+
 // AH_FLASH_BWD=onepass makes variant 1 of the backward pass the default of a process (measurement aid)
 bool flash_bwd_one_pass() {
   static const bool on = [] { const char *e = getenv("AH_FLASH_BWD"); return e && strcmp(e, "onepass") == 0; }();
@@ -45,6 +51,29 @@ __device__ __forceinline__ void tile_load(const uint16_t *__restrict__ base, int
     if (row0 + r < T && (!PAD || c8 * 8 < hd)) x = *reinterpret_cast<const u32x4 *>(base + (int64_t)(row0 + r) * st + c8 * 8);
     v[i] = x;
   }
+}
+template <int D>
+__device__ __forceinline__ void tile_store(uint16_t *s, const u32x4 (&v)[Geo<D>::CHUNKS]) {
+#pragma unroll
+  for (int i = 0; i < Geo<D>::CHUNKS; i++) {
+    int c = threadIdx.x + 256 * i, r = c / (D / 8), c8 = c % (D / 8);
+    *reinterpret_cast<u32x4 *>(s + r * Geo<D>::PITCH + c8 * 8) = v[i];
+  }
+}
+// A/B fragment with the tile ROW as the MFMA row/column (k = feature d): rows r0 + lane%32, d = 16*ks + 8*(lane/32)..
+template <int D>
+__device__ __forceinline__ bf16x8 tile_frag(const uint16_t *s, int r0, int ks, int lane) {
+  return *reinterpret_cast<const bf16x8 *>(s + (r0 + (lane & 31)) * Geo<D>::PITCH + ks * 16 + (lane >> 5) * 8);
+}
+// A fragment with the feature d as the MFMA row (k = tile row, in the accumulator's slot order): features
+// 32*db + lane%32, k-slot i of this half = tile row r0 + 16m + 8(i/4) + 4(lane/32) + i%4.
+template <int D>
+__device__ __forceinline__ bf16x8 tile_frag_t(const uint16_t *s, int r0, int m, int db, int lane) {
+  int j = lane & 15, g = lane >> 4, lk = g >> 1;
+  const uint16_t *p = s + (r0 + 16 * m + 4 * lk + (j >> 2)) * Geo<D>::PITCH + 32 * db + 16 * (g & 1) + 4 * (j & 3);
+  bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)p);
+  bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4 *)(p + 8 * Geo<D>::PITCH));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // this lane's row of a [T][D] operand as B fragments (k = d): one 16-byte global load per 16 features
 template <int D, bool PAD = false>
