@@ -1,7 +1,7 @@
 """Per-op microbenchmarks on the shapes of the training step, in the manner of the reference's scripts/bench-ops.ts
 (3 warm-up calls, then the mean of `iters` calls; TFLOP/s = flops / time, GB/s = algorithmic bytes / time):
 
-    python -m alpha2_amd.bench_ops [--iters 10] [--only gemm|flash|bandwidth|ceiling|epilogue|issue] [--json]
+    python -m alpha2_amd.bench_ops [--iters 10] [--only gemm|flash|bandwidth|ceiling|epilogue|issue|generation] [--json]
 
 * GEMM: C = A B^T and both backward products, M = 16384 (batch x context), K = 768, N in {768, 2304, 3072, 50304},
   bf16 operands with fp32 accumulation and fp32 throughout; flops 2 M N K (scripts/bench-ops.ts:302,328).
@@ -18,8 +18,10 @@
 * `--only issue` (not part of the default run): what one SIMD issues per nanosecond (`ah_probe_issue`: v_fma_f32, v_exp_f32, a
   mix of the two, an MFMA alone and with vector work behind it, at one, two and four waves per SIMD): the figures the
   attention kernels, whose time goes to per-score vector instructions, are read against.
+* `--only generation` (not part of the default run): `sampleTokensBatch` on a GPT-2-small shape, tokens behind prompts of 20 to 400, in fp32 (against
+  `sampleTokens` on four of the prompts, scaled to all) and on the fast backend; by the host's clock, whole calls.
 
-Every call goes through the C ABI; timing is by HIP events on the library's stream.  Peaks used for the last column:
+Every call but those of generation goes through the C ABI; timing is by HIP events on the library's stream.  Peaks used for the last column:
 2.5 PFLOP/s (bf16 MFMA), a sixth of it (fp32 products: six bf16 products each), 8 TB/s (HBM).
 """
 from __future__ import annotations
@@ -29,10 +31,13 @@ import ctypes as C
 import json
 import math
 import sys
+import time
 
 import numpy as np
 
-from . import HipBackend, _ffi as ffi
+from . import FastHipBackend, HipBackend, SeededRng, _ffi as ffi
+from .model import ModelConfig, initGPT
+from .sample import SampleConfig, sampleTokens, sampleTokensBatch
 
 PEAK_TFLOPS = {"bf16": 2500.0, "f32": 2500.0 / 6}
 PEAK_GBS = 8000.0
@@ -325,15 +330,42 @@ def bench_issue(b: Bench):
             print(f"{name:40s} {waves:10d} {ns:22.2f}", flush=True)
 
 
+def bench_generation(b: Bench, prompts=(1, 16, 64), steps: int = 32, vocab: int = 50304, layers: int = 12, width: int = 768, heads: int = 12):
+    """Several prompts at once and, in fp32, one after the other."""
+    cfg = ModelConfig(vocabSize=vocab, blockSize=1024, nLayer=layers, nEmbd=width, nHead=heads)
+    options = SampleConfig(steps=steps, temperature=0.8, topk=40)
+
+    def clock(fn) -> float:
+        fn()                                                    # (warm: kernels loaded, blocks in the pool)
+        begun = time.perf_counter()
+        fn()
+        return (time.perf_counter() - begun) * 1e3
+
+    for backend in (b.B, FastHipBackend(0)):
+        params = initGPT(cfg, backend, SeededRng(1))
+        rs = np.random.RandomState(0)
+        for n in prompts:
+            texts = [rs.randint(0, vocab, rs.randint(20, 400)).tolist() for _ in range(n)]
+            call = (options, backend.releaseGpuTensor, backend.flush)
+            row = {"op": f"generation {type(backend).__name__}", "prompts": n, "steps": steps,
+                   "ms": clock(lambda: sampleTokensBatch(cfg, params, backend, [SeededRng(i) for i in range(n)], texts, *call))}
+            if backend is b.B:
+                some = texts[:4]
+                row["ms_one_by_one"] = clock(lambda: [sampleTokens(cfg, params, backend, SeededRng(i), t, *call) for i, t in enumerate(some)]) * n / len(some)
+            b.rows.append(row)
+            print(f"{row['op']:34s} {n:4d} prompts, {steps} tokens each: {row['ms']:8.1f} ms"
+                  + (f", one by one {row['ms_one_by_one']:8.1f} ms" if "ms_one_by_one" in row else ""), flush=True)
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--iters", type=int, default=10)
-    ap.add_argument("--only", choices=["gemm", "flash", "bandwidth", "ceiling", "epilogue", "issue"])
+    ap.add_argument("--only", choices=["gemm", "flash", "bandwidth", "ceiling", "epilogue", "issue", "generation"])
     ap.add_argument("--json", action="store_true", help="also print one JSON line with every row")
     args = ap.parse_args(argv)
     b = Bench(args.iters)
-    if args.only == "issue":
-        bench_issue(b)
+    if args.only in ("issue", "generation"):
+        (bench_issue if args.only == "issue" else bench_generation)(b)
         if args.json:
             print(json.dumps(b.rows))
         return 0

@@ -26,3 +26,13 @@ def test_op_microbenchmarks_run_and_report_sane_rates(capsys):
     by = {r["op"]: r for r in rows}
     assert by["gemm bf16 N=3072 fwd  C=A.B^T"]["tflops"] > 300          # far below the measured 980: a broken dispatch, not noise
     assert by["adamw 163.0M (+bf16 shadow)"]["gbs"] > 2000
+
+
+@pytest.mark.gpu
+def test_generation_is_timed_with_and_without_the_batch(capsys):
+    from alpha2_amd import bench_ops
+    b = bench_ops.Bench(1)
+    bench_ops.bench_generation(b, prompts=(1, 5), steps=3, vocab=97, layers=1, width=64, heads=2)
+    assert [(r["op"].split()[1], r["prompts"], r["ms"] > 0, r.get("ms_one_by_one", 0) > 0) for r in b.rows] == [
+        ("HipBackend", 1, True, True), ("HipBackend", 5, True, True), ("FastHipBackend", 1, True, False), ("FastHipBackend", 5, True, False)]
+    assert capsys.readouterr().out.count("prompts") == 4
