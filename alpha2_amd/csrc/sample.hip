@@ -243,12 +243,14 @@ struct Weight {
   uint64_t each;                                 // 0, or what each of them counts
   __device__ __forceinline__ uint64_t operator()(float l) const {
     if (each) return each;
-    const double y = ((double)l - (double)top) * factor;
-    const bool some = y > -44.0 * STEPS;         // (not NaN)
+    // y = below * factor.  Written with fma and not with y: a compiler that fuses the two in one of this function's many places and not in another would give a
+    // logit two weights, and running sums that no total agrees with.
+    const double below = (double)l - (double)top;
+    const bool some = below * factor > -44.0 * STEPS;                // (not NaN)
     constexpr double ROUND = 0x1.8p52;
-    const double whole = y + ROUND;
+    const double whole = fma(below, factor, ROUND);
     const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, whole);
-    const double g = (y - (whole - ROUND)) * (0.693147180559945309417 / STEPS);
+    const double g = fma(below, factor, -(whole - ROUND)) * (0.693147180559945309417 / STEPS);
     const float h = (float)g;
     const double e = fma(g * g, (double)fmaf(h, fmaf(h, 1.0f / 24, 1.0f / 6), 0.5f), g);
     const double step = steps[n & (STEPS - 1)], w = fma(step, e, step);
