@@ -151,7 +151,9 @@ class PagedContext:
     @staticmethod
     def of(cfg: ModelConfig, params: dict, backend, longest: Sequence[int]) -> Optional["PagedContext"]:
         """For sequences of at most `longest` tokens each.  None where each has to be run by itself: another backend or wiring of
-        attention, a head size that the kernels do not take, or no memory for the keys and values."""
+        attention, a head size that the kernels do not take, no memory for the keys and values, or nothing to keep."""
+        if max(longest, default=0) < 1:
+            return None
         if not isinstance(backend, HipBackend) or cfg.attention != "heads" or cfg.dropout != 0:
             return None
         if cfg.nEmbd % cfg.nHead or not flashHeadSize(cfg.nEmbd // cfg.nHead) or cfg.vocabSize > 1 << 20 or max(longest) > cfg.blockSize:

@@ -219,3 +219,9 @@ def test_fewer_than_no_steps(monkeypatch):
         for steps in ([-1, 3], [0, -5]):
             with pytest.raises(ValueError, match="steps"):
                 sampleTokensBatch(ModelConfig(**CFG), {}, OneTokenEach(), [Draw(), Draw(0.1, 0.2, 0.3)], [[1, 2], [3]], [SampleConfig(steps=n) for n in steps])
+
+
+@pytest.mark.parametrize("longest", [[], [0], [0, 0]])
+def test_no_sequences_or_none_with_a_token(longest):
+    params = {"layers": [{}], "wpe": type("V", (), {"data": T(12, 16)})()}
+    assert PagedContext.of(ModelConfig(**CFG), params, HipBackend.__new__(HipBackend), longest) is None
