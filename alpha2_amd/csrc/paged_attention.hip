@@ -4,11 +4,14 @@
 //   x_j = scale q.k_j (capped: cap tanh(x_j / cap)),  o = sum_j e^(x_j - m) v_j / sum_j e^(x_j - m),  lse = m + log sum_j e^(x_j - m)
 // in one pass over j with the running maximum m, sum l and product o, all in fp32; where the positions are cut into parts, each part leaves
 // its (m, l, o) and a second kernel joins them: m = max m_i, l = sum l_i e^(m_i - m), o = sum o_i e^(m_i - m).
+// bf16 pages: a weight e^(x_j - m) is rounded to bf16 for the product with v_j, which is what the matrix instructions take (as in attention_bf16.hip; fp32 products would be
+// at an eighth of their rate), and goes into l as it was.  Outputs are 2.2e-3 off 64 bits (root mean square, relative), 1.7e-3 of them by their own rounding.
 //
 // Work.  The heads that share keys are rows of one matrix: a COLUMN is a (new token, head of the group), column i of a sequence token
 // i / group, head i % group.  A workgroup takes one unit: TILE columns of a sequence, one kv head, one part of the positions.  Which unit that is
-// follows from starts and lens on the device (find_unit), so the lengths need not be known on the host, ragged batches are cut evenly
-// (parts are as long as the launch's work over the workgroups wanted, and those of a sequence as long as each other) and a captured launch follows them.
+// follows from starts and lens on the device (find_unit), so the lengths need not be known on the host and a captured launch follows them.  Where tiles are few the positions
+// are cut (parts as long as the launch's work over the workgroups wanted, those of a sequence as long as each other), so that contexts of any lengths end together; where the
+// tiles alone are as many as the GPU takes at once, nothing is, however much longer than the others one context is (attend).
 //
 // Two kernels for each type; both compute every case, which is taken is a matter of speed (ah_paged_attention):
 //   keys   16 columns; the four waves take tiles of positions in turn and are joined in LDS.  For one or a few new tokens a sequence, where the
@@ -63,7 +66,9 @@ __device__ __forceinline__ int parts_of(const Sequence &s, const PagedCache &c, 
   return reach <= plan.whole ? 1 : parts_of(reach, span);
 }
 
-// Unit `index` of the launch, or (by_tile) tile `index`, by a whole wave; the same for all its lanes.  A lane looks at a sequence.
+// Unit `index` of the launch, or (by_tile) tile `index`, by a whole wave; the same for all its lanes.  A lane looks at a sequence, and every workgroup at all of
+// them: what that takes grows with the square of their number.  A token each after 64 positions, 8 heads of 64 on 1: 192 sequences 7.5 us, 1024 19, 4096 146, 16384 1900
+// (their bytes 0.8, 4, 16 and 65).
 template <int TILE>
 __device__ __forceinline__ Unit find_unit(const PagedCache &c, const Plan &plan, int group, int index, bool by_tile) {
   const int lane = threadIdx.x & 63;
@@ -974,7 +979,8 @@ constexpr int64_t PART_BYTES = int64_t(60) << 20;
 
 // TILE columns to a unit: how many workgroups, and how many of them the positions are cut for.  Two workgroups fit a compute unit; where the tiles alone
 // are as many, nothing is cut (64 sequences of 1024, 8 kv heads of 128, bf16: 44 us, 53 us cut), and the join is not launched either where the table
-// cannot name more positions than a part has.  Otherwise about `wanted` units are cut: more of them even out ragged sequences, fewer are fewer to join.
+// cannot name more positions than a part has.  That rule sees no lengths: 63 sequences of 500 beside one of 24000, the same heads, take 477 us, the one by itself 29, and 47
+// beside it, which are cut, 53; 15 of 300 beside one of 32768, 32 kv heads, 656 us, the one by itself 109.  Otherwise about `wanted` units are cut: more of them even out ragged sequences, fewer are fewer to join.
 template <class T, int TILE, int D, class Kernel>
 int32_t attend(AttendArgs a, Kernel kernel, int64_t wanted, int32_t least, int32_t whole) {
   // of one kv head, at most: every sequence with new tokens may end inside a tile
@@ -1010,6 +1016,9 @@ template <int D>
 int32_t attend_sized(const AttendArgs &a, bool bf16_pages) {
   // Columns of a sequence, in the mean.  At 32 the two are even (bf16, 4 x 8192 positions, 8 kv heads of 128: 40 and 39 us; fp32, 4 x 1024, 12 of 64: 19.0
   // and 19.6); at 48, 60 and 44 us; at 256, 182 and 74.  The other way, 16 columns: 35 and 39 us.
+  // The mean is the launch's, so a prompt beside single tokens may go through tiles of 16 columns, or they through its own.  bf16, 8 heads of 128, 63 tokens after 500 positions
+  // and a prompt of 1900 (keys) 73 us, of 2048 (rows) 78, in two calls 25 and 38; on 32 heads, 41 (400 new, keys), 44 (600, rows) and 82 (2048), in two 26 and 22, 33, 66.
+  // Sequences without new tokens count: a chunk of 2048 in 8192 positions, 8 heads of 128, 86 us, beside 62 idle ones, with fewer parts, 215, beside 63 (keys) 291.
   const bool rows = (int64_t)a.c.rows * a.group > (int64_t)32 * a.c.seqs;
   const int64_t cus = num_cus();
   // Units wanted, of keys: three to a compute unit, 246 us at 24 ragged sequences of up to 24000 positions (8 kv heads of 128, bf16), two, 276, four, 245; at

@@ -146,7 +146,7 @@ class PagedContext:
     where they lie may change from call to call."""
 
     PAGE = 64               # positions to a page
-    MOST_ROWS = 8192        # tokens of one pass that a caller should give it, for the memory that its activations take
+    MOST_ROWS = 8192        # prompts' tokens of one pass that a caller should give it, for the memory that its activations take (a step has a token of every sequence)
 
     @staticmethod
     def of(cfg: ModelConfig, params: dict, backend, longest: Sequence[int]) -> Optional["PagedContext"]:

@@ -135,9 +135,11 @@ def sampleTokens(config: ModelConfig, params: dict, backend, rng, promptTokens: 
 
 def sampleTokensBatch(config: ModelConfig, params: dict, backend, rngs: Sequence, prompts: Sequence[Sequence[int]], sampleConfigs,
                       releaseTensor: Optional[Callable] = None, flushGpu: Optional[Callable] = None) -> List[np.ndarray]:
-    """What sampleTokens returns for each prompt with its own rng (and, from a sequence of SampleConfig, its own options): a sequence's
-    tokens do not depend on which others are run with it, but for sums taken in other orders.  One forward pass serves a token of every
-    sequence; where model or backend do not allow that, the sequences are run one after the other."""
+    """What sampleTokens returns for each prompt with its own rng (and, from a sequence of SampleConfig, its own options), but for roundings: sums are
+    taken in other orders, which depend on the sequences that are run together, and the selection on the device takes draws and options in 32
+    bits where sampleTokens has 64 (of a full softmax over 50304 tokens a draw falls on the other side of a border about once in two thousand, by
+    estimate).  Prompts that share an rng draw from it in turn, token by token.  One forward pass serves a token of every sequence; where model
+    or backend do not allow that, the sequences are run one after the other."""
     prompts = [np.asarray(p, dtype=np.int32).reshape(-1) for p in prompts]
     configs = [sampleConfigs] * len(prompts) if isinstance(sampleConfigs, SampleConfig) else list(sampleConfigs)
     if len(rngs) != len(prompts) or len(configs) != len(prompts):

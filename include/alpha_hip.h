@@ -503,7 +503,9 @@ int32_t ah_decode_next_ticks(int32_t ticks);
  *      A page may be shared by sequences; two new tokens must not fall on one row of a page, and starts must not fall.
  *      All pointers 16-byte aligned (table, starts, lens, lse: 4), strides multiples of 16 bytes and below 2^31 times 16 bytes; head_dim a
  *      multiple of 8 from 8 to 128.  Positions from 0x7fff0000 on count as past the table.
- *      Attention leaves parts of long contexts in the library's scratch, so it belongs on the main stream like all that uses that. ---- */
+ *      Attention leaves parts of long contexts in the library's scratch, so it belongs on the main stream like all that uses that.
+ *      How contexts are cut is decided by their number: where sequences times kv_heads come to twice the compute units, one that is many times
+ *      longer than the others is faster in a call of its own; and few long chunks are faster without sequences that have no new tokens. ---- */
 typedef struct {
   int32_t dtype;                 /* AH_F32 or AH_BF16: of the pages and of every q, k, v and o that meets them */
   int32_t kv_heads, head_dim;
