@@ -193,6 +193,8 @@ class HipBackend:
         if t._buf is None or not t._dev_valid:
             if not t._host_valid:
                 raise RuntimeError("use of a released tensor")
+            if t._host.size != t.size:                          # kernels go by the shape
+                raise ValueError(f"{t._host.size} values in the host's memory for a tensor of {t.shape}")
             rounded = t.store != t.dtype                        # host contents are f32: stored in bf16, they are read back as that
             host = _bf16_bits(t._host) if rounded else t._host
             if t._buf is None:

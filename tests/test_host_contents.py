@@ -1,4 +1,4 @@
-"""Host contents given to a tensor that is stored in bf16 (a page of keys filled by hand, a cached activation put back): what is uploaded, and how much."""
+"""Host contents given to a tensor: as many as its shape says, and in bf16 where it is stored so (a page of keys filled by hand, a cached activation put back)."""
 import ctypes as C
 
 import numpy as np
@@ -78,3 +78,32 @@ def test_other_storage_is_uploaded_as_it_is(backend, dtype):
     ptr = backend._ptr(t)
     block, room = backend.lib.blocks[ptr]
     assert room == 12 and block[:12].view(t.data.dtype).tolist() == [1, -2, 3] and t._host_valid
+
+
+@pytest.mark.parametrize("dtype,store", [("i32", "i32"), ("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("n", [0, 5, 7, 13])
+def test_host_contents_of_another_size_are_refused(backend, dtype, store, n):
+    """A kernel goes by the shape: a table, a list of tokens or a page with fewer numbers than that would be read past its end, with more written past its block's."""
+    t = TensorData((2, 3), dtype, np.zeros(n))
+    t.store = store
+    with pytest.raises(ValueError, match=r"\(2, 3\)"):
+        backend._ptr(t)
+    t = backend._new((2, 3), dtype, store)
+    t.data = np.zeros(n)
+    with pytest.raises(ValueError, match=r"\(2, 3\)"):
+        backend._ptr(t)
+    assert backend.lib.uploads == []
+    t.data = np.arange(6)
+    backend._ptr(t)
+    assert t.data.tolist() == [0, 1, 2, 3, 4, 5]
+
+
+def test_tokens_of_another_number_than_asked_for(backend):
+    from alpha2_amd.decode import PagedContext
+    from alpha2_amd.model import ModelConfig
+    kept = PagedContext(ModelConfig(vocabSize=20, blockSize=12, nLayer=0, nEmbd=16, nHead=2), {"wte": type("V", (), {"data": TensorData((20, 16), "f32", np.zeros(320)), "requiresGrad": False})()}, backend, [12])
+    backend.lib.ah_embedding = lambda *a: pytest.fail("the kernel has been called")
+    for tokens in (np.zeros(2, np.int32), np.zeros(4, np.int32), TensorData((2,), "i32", np.zeros(2))):
+        with pytest.raises(ValueError):
+            kept.forward([0], [3], tokens, [0], None)
+    assert kept.lens.tolist() == [0]
